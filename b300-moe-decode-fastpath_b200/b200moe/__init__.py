@@ -11,6 +11,7 @@ from .forward import ARCHITECTURE, b300_moe_forward, b300_moe_forward_pinned
 from .fp8 import (Fp8ExpertWeights, b300_moe_forward_fp8, dequantize_expert_weights_fp8,
                   dequantize_rows_fp8, quantize_expert_weights_fp8, quantize_rows_fp8)
 from .graphed import GraphedMoEDecodeLayer
+from .norm import add_rms_norm, add_rms_norm_fp8
 from .nvfp4 import (Nvfp4ExpertWeights, b300_moe_forward_nvfp4, prepared_nvfp4_weights,
                     quantize_expert_weights_nvfp4)
 from .ops import DispatchResult, combine_tokens, dispatch_tokens
@@ -28,6 +29,8 @@ __all__ = [
     "Nvfp4ExpertWeights",
     "RoutedMoEShape",
     "StagedLayer",
+    "add_rms_norm",
+    "add_rms_norm_fp8",
     "b300_moe_forward",
     "b300_moe_forward_fp8",
     "b300_moe_forward_nvfp4",

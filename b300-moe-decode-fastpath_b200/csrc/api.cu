@@ -141,6 +141,10 @@ cudaError_t launch_ep_combine_push(const int64_t* reverse_mapping, const void* w
 cudaError_t launch_router_topk(const void* logits, bool logits_f32, int num_tokens,
                                int num_experts, int top_k, int64_t* ids, void* weights_bf16,
                                float* weights_f32, cudaStream_t stream);
+cudaError_t launch_add_rms_norm(const void* x, const void* residual, bool residual_f32,
+                                const void* weight, bool weight_f32, long long rows, int hidden,
+                                float eps, void* out, uint8_t* codes, float* scale,
+                                void* residual_out, cudaStream_t stream);
 
 extern int g_gemm_stage_kb;
 extern int g_gemm_evict_first;
@@ -818,6 +822,29 @@ int b200moe_fp8_dequantize_rows(const uint8_t* q, const float* scale, long long 
   if (rc) return rc;
   return (int)launch_fp8_dequantize_rows(q, scale, rows, cols, out_bf16,
                                          static_cast<cudaStream_t>(stream));
+}
+
+int b200moe_add_rms_norm(const void* hidden, const void* residual, int residual_is_f32,
+                         const void* weight, int weight_is_f32, long long rows, int hidden_size,
+                         float eps, void* out_bf16, uint8_t* codes_out, float* scale_out,
+                         void* residual_out, void* stream) {
+  if (!hidden || !weight || (out_bf16 == nullptr) == (codes_out == nullptr) ||
+      (codes_out == nullptr) != (scale_out == nullptr) ||
+      (residual == nullptr) != (residual_out == nullptr))
+    return B200MOE_E_NULL;
+  if (rows < 1 || rows > 0x7fffffffll || hidden_size < 8 ||
+      hidden_size > B200MOE_NORM_MAX_HIDDEN || !(eps >= 0.0f))
+    return B200MOE_E_SHAPE;
+  if (hidden_size % (codes_out ? 16 : 8) || !aligned16(hidden) || !aligned16(residual) ||
+      !aligned16(weight) || !aligned16(out_bf16) || !aligned16(codes_out) ||
+      !aligned16(residual_out))
+    return B200MOE_E_ALIGN;
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc) return rc;
+  return (int)launch_add_rms_norm(hidden, residual, residual_is_f32 != 0, weight,
+                                  weight_is_f32 != 0, rows, hidden_size, eps, out_bf16, codes_out,
+                                  scale_out, residual_out, static_cast<cudaStream_t>(stream));
 }
 
 int b200moe_tune(int knob, int value) {

@@ -491,6 +491,27 @@ int b200moe_router_topk(const void* logits, int logits_are_f32, int num_tokens, 
                         float* weights_f32, void* stream);
 
 /*
+ * Residual addition and root-mean-square norm of token rows (the step in front of the layer),
+ * one kernel.  No counterpart in the reference.  Per row: s = hidden + residual in FP32,
+ * residual_out = s in the residual's type, y = s * weight / sqrt(mean(s^2) + eps).
+ *   hidden            [rows,H] bf16
+ *   residual          [rows,H] bf16, or fp32 when residual_is_f32 != 0; NULL: s = hidden and
+ *                     residual_out must be NULL too
+ *   weight            [H] bf16, or fp32 when weight_is_f32 != 0
+ *   out_bf16          [rows,H] bf16 out, or NULL when the result is wanted in 8 bits:
+ *   codes_out, scale_out   [rows,H] E4M3 bytes and [rows] fp32 out, the format and rule of
+ *                     b200moe_fp8_quantize_rows applied to the FP32 values y; else both NULL
+ * out_bf16 and residual_out may be `hidden` or `residual` themselves (same type); no other
+ * overlap.  H <= B200MOE_NORM_MAX_HIDDEN, a multiple of 8 (16 for codes); pointers 16-byte
+ * aligned (scale_out 4).
+ */
+#define B200MOE_NORM_MAX_HIDDEN 32768
+int b200moe_add_rms_norm(const void* hidden, const void* residual, int residual_is_f32,
+                         const void* weight, int weight_is_f32, long long rows, int hidden_size,
+                         float eps, void* out_bf16, uint8_t* codes_out, float* scale_out,
+                         void* residual_out, void* stream);
+
+/*
  * Process-wide tuning knobs of the grouped GEMMs, for benchmarking sweeps.  No
  * counterpart in the reference (its GEMMs are library calls with no knobs).
  * Not thread-safe against concurrent forwards; results never depend on them.
