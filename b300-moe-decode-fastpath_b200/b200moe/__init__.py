@@ -11,6 +11,7 @@ from .forward import ARCHITECTURE, b300_moe_forward, b300_moe_forward_pinned
 from .fp8 import (Fp8ExpertWeights, b300_moe_forward_fp8, dequantize_expert_weights_fp8,
                   dequantize_rows_fp8, quantize_expert_weights_fp8, quantize_rows_fp8)
 from .graphed import GraphedMoEDecodeLayer
+from .layer import b300_moe_layer, b300_moe_layer_fp8
 from .norm import add_rms_norm, add_rms_norm_fp8
 from .nvfp4 import (Nvfp4ExpertWeights, b300_moe_forward_nvfp4, prepared_nvfp4_weights,
                     quantize_expert_weights_nvfp4)
@@ -35,6 +36,8 @@ __all__ = [
     "b300_moe_forward_fp8",
     "b300_moe_forward_nvfp4",
     "b300_moe_forward_pinned",
+    "b300_moe_layer",
+    "b300_moe_layer_fp8",
     "build_info",
     "combine_tokens",
     "cuda_extension_available",

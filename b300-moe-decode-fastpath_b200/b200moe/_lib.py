@@ -73,6 +73,7 @@ EXPORTS = (
     "b200moe_router_topk",
     "b200moe_fp8_quantize_rows",
     "b200moe_fp8_dequantize_rows",
+    "b200moe_layer",
     "b200moe_add_rms_norm",
 )
 
@@ -252,6 +253,9 @@ def _declare(lib: ctypes.CDLL) -> None:
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p,
         ctypes.c_void_p,
     ]
+    lib.b200moe_layer.restype = ctypes.c_int
+    lib.b200moe_layer.argtypes = [args_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+                                  ctypes.c_void_p, ctypes.c_void_p]
     lib.b200moe_add_rms_norm.restype = ctypes.c_int
     lib.b200moe_add_rms_norm.argtypes = [
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,

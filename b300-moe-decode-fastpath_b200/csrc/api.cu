@@ -145,6 +145,12 @@ cudaError_t launch_add_rms_norm(const void* x, const void* residual, bool residu
                                 const void* weight, bool weight_f32, long long rows, int hidden,
                                 float eps, void* out, uint8_t* codes, float* scale,
                                 void* residual_out, cudaStream_t stream);
+cudaError_t launch_layer_few(const void* x, const void* router, bool router_f32,
+                             const void* gate_up, const void* down, const float* gate_up_scale,
+                             const float* down_scale, int tokens, int hidden, int inter,
+                             int experts, int top_k, double* logits, void* act_hi, void* act_lo,
+                             void* out, int64_t* ids_out, float* weights_out, unsigned int* sync,
+                             uint32_t* status, int sm_count, cudaStream_t stream);
 
 extern int g_gemm_stage_kb;
 extern int g_gemm_evict_first;
@@ -721,7 +727,7 @@ const char* b200moe_error_string(int code) {
     case B200MOE_E_LIMIT:
       return "the call exceeds a fixed limit of this entry point (b200moe_routing_static: "
              "4096 assignments; b200moe_ep_combine_reduce with B200MOE_FLAG_EP_PUSH: a grid "
-             "that is resident at once)";
+             "that is resident at once; b200moe_layer: 8 tokens, H <= 8192, I <= 65536)";
     default: break;
   }
   if (code > 0) return cudaGetErrorString((cudaError_t)code);
@@ -822,6 +828,37 @@ int b200moe_fp8_dequantize_rows(const uint8_t* q, const float* scale, long long 
   if (rc) return rc;
   return (int)launch_fp8_dequantize_rows(q, scale, rows, cols, out_bf16,
                                          static_cast<cudaStream_t>(stream));
+}
+
+int b200moe_layer(const B200MoeArgs* a, const void* router_weight, int router_is_f32,
+                  int64_t* indices_out, float* weights_out, void* stream) {
+  if (!a || !a->hidden_states || !router_weight || !a->gate_up_weight || !a->down_weight ||
+      !a->swiglu_output || !a->output)
+    return B200MOE_E_NULL;
+  if (a->flags & ~(uint32_t)(B200MOE_FLAG_PDL | B200MOE_FLAG_FP8_WEIGHTS))
+    return B200MOE_E_UNSUPPORTED;
+  if (a->num_tokens > B200MOE_LAYER_MAX_TOKENS || a->hidden_size > B200MOE_LAYER_MAX_HIDDEN ||
+      a->intermediate_size > B200MOE_LAYER_MAX_INTER)
+    return B200MOE_E_LIMIT;
+  Ctx c;
+  int rc = prepare(a, stream, &c);
+  if (rc) return rc;
+  const bool fp8 = fp8_weights(a);
+  if (fp8 && (!a->gate_up_scale || !a->down_scale)) return B200MOE_E_NULL;
+  if (fp8 && (a->hidden_size % 16 || a->intermediate_size % 16)) return B200MOE_E_ALIGN;
+  if (!aligned16(a->hidden_states) || !aligned16(router_weight) || !aligned16(a->gate_up_weight) ||
+      !aligned16(a->down_weight) || !aligned16(a->swiglu_output))
+    return B200MOE_E_ALIGN;
+  const ScratchLayout l =
+      scratch_layout(a->rows_cap, a->num_experts, a->hidden_size, a->intermediate_size);
+  char* base = static_cast<char*>(a->scratch);
+  return (int)launch_layer_few(
+      a->hidden_states, router_weight, router_is_f32 != 0, a->gate_up_weight, a->down_weight,
+      fp8 ? a->gate_up_scale : nullptr, fp8 ? a->down_scale : nullptr, a->num_tokens,
+      a->hidden_size, a->intermediate_size, a->num_experts, a->top_k,
+      reinterpret_cast<double*>(base + l.few_logits), a->swiglu_output, base + l.act_lo, a->output,
+      indices_out, weights_out, reinterpret_cast<unsigned int*>(base + kFewSyncOffsetBytes),
+      reinterpret_cast<uint32_t*>(base + l.status), c.dev.sm_count, c.stream);
 }
 
 int b200moe_add_rms_norm(const void* hidden, const void* residual, int residual_is_f32,

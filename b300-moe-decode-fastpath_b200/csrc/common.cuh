@@ -134,8 +134,14 @@ struct ScratchLayout {
   size_t x_scale;    // fp32 [rows_cap]
   size_t a_scale;    // fp32 [rows_cap]
   size_t a_amax;     // uint32 [rows_cap]  bit pattern of max |activation| per row
+  size_t few_logits; // fp64 [kFewMaxTokens, experts]  b200moe_layer only
   size_t total;
 };
+
+// The whole layer in one kernel (b200moe_layer): most tokens of a call, and where its three
+// grid-barrier counters lie in the status area (behind the timeline words, zero between calls)
+constexpr int kFewMaxTokens = B200MOE_LAYER_MAX_TOKENS;
+constexpr size_t kFewSyncOffsetBytes = 192;
 
 constexpr int kNvfp4Planes = 4;      // E2M1 planes per token row of the NVFP4-weight path
 constexpr int kSegRowsNvfp4 = 64;    // its longest segment: four planes of 64 rows, N = 64 per MMA
@@ -157,7 +163,9 @@ __host__ __device__ inline ScratchLayout scratch_layout(int rows_cap, int expert
   l.x_scale = align_up(l.q_planes + (size_t)kFp8Planes * rows_cap * widest, kScratchAlign);
   l.a_scale = align_up(l.x_scale + (size_t)rows_cap * sizeof(float), kScratchAlign);
   l.a_amax = align_up(l.a_scale + (size_t)rows_cap * sizeof(float), kScratchAlign);
-  l.total = align_up(l.a_amax + (size_t)rows_cap * sizeof(uint32_t), kScratchAlign);
+  l.few_logits = align_up(l.a_amax + (size_t)rows_cap * sizeof(uint32_t), kScratchAlign);
+  l.total = align_up(l.few_logits + (size_t)kFewMaxTokens * experts * sizeof(double),
+                     kScratchAlign);
   return l;
 }
 

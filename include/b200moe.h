@@ -491,6 +491,28 @@ int b200moe_router_topk(const void* logits, int logits_are_f32, int num_tokens, 
                         float* weights_f32, void* stream);
 
 /*
+ * The whole layer for a few tokens in ONE kernel, router included: logits = hidden x
+ * router_weight^T, the top_k largest per token (lower id first among equal ones, NaN above every
+ * number), softmax over them, gate+up, SwiGLU, down and the weighted sum.  No counterpart in the
+ * reference.  For T <= B200MOE_LAYER_MAX_TOKENS; b200moe_forward takes larger calls.
+ *   args          hidden_states, gate_up_weight, down_weight (and the two row scales with
+ *                 B200MOE_FLAG_FP8_WEIGHTS, then H and I divisible by 16), the dimensions,
+ *                 rows_cap, swiglu_output, scratch, output; flags 0 or
+ *                 B200MOE_FLAG_FP8_WEIGHTS, B200MOE_FLAG_PDL (no effect).  All on the device.
+ *   router_weight [E,H] bf16, or fp32 when router_is_f32 != 0
+ *   indices_out   [T,K] int64 out or NULL
+ *   weights_out   [T,K] fp32 out or NULL: the softmax weights, which are used unrounded
+ * The first 256 bytes of scratch must be zero before the first call on it (they hold the
+ * grid-barrier counters, which every call leaves at zero, and the status word).  A cooperative
+ * launch of one block per SM; one scratch serves one call at a time.
+ */
+#define B200MOE_LAYER_MAX_TOKENS 8
+#define B200MOE_LAYER_MAX_HIDDEN 8192
+#define B200MOE_LAYER_MAX_INTER  65536
+int b200moe_layer(const B200MoeArgs* args, const void* router_weight, int router_is_f32,
+                  int64_t* indices_out, float* weights_out, void* stream);
+
+/*
  * Residual addition and root-mean-square norm of token rows (the step in front of the layer),
  * one kernel.  No counterpart in the reference.  Per row: s = hidden + residual in FP32,
  * residual_out = s in the residual's type, y = s * weight / sqrt(mean(s^2) + eps).
