@@ -17,6 +17,7 @@ from .nvfp4 import (Nvfp4ExpertWeights, b300_moe_forward_nvfp4, prepared_nvfp4_w
                     quantize_expert_weights_nvfp4)
 from .ops import DispatchResult, combine_tokens, dispatch_tokens
 from .router import topk_routing
+from .sampling import sample_tokens
 from .stages import StagedLayer
 from .validation import RoutedMoEShape, validate_routed_moe_inputs
 from .workspace import B300MoEWorkspace
@@ -48,6 +49,7 @@ __all__ = [
     "quantize_expert_weights_fp8",
     "quantize_expert_weights_nvfp4",
     "quantize_rows_fp8",
+    "sample_tokens",
     "topk_routing",
     "validate_routed_moe_inputs",
 ]

@@ -74,6 +74,7 @@ EXPORTS = (
     "b200moe_fp8_quantize_rows",
     "b200moe_fp8_dequantize_rows",
     "b200moe_layer",
+    "b200moe_sample",
     "b200moe_add_rms_norm",
 )
 
@@ -256,6 +257,13 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.b200moe_layer.restype = ctypes.c_int
     lib.b200moe_layer.argtypes = [args_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
                                   ctypes.c_void_p, ctypes.c_void_p]
+    lib.b200moe_sample.restype = ctypes.c_int
+    lib.b200moe_sample.argtypes = [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p,
+    ]
     lib.b200moe_add_rms_norm.restype = ctypes.c_int
     lib.b200moe_add_rms_norm.argtypes = [
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,

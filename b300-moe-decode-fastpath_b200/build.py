@@ -22,7 +22,7 @@ CSRC = PACKAGE_ROOT / "csrc"
 INCLUDE = PACKAGE_ROOT.parent / "include"
 SOURCES = ("api.cu", "routing.cu", "rows.cu", "grouped_gemm.cu", "grouped_gemm_fp8.cu",
            "grouped_gemm_nvfp4.cu", "quant.cu", "nvfp4_quant.cu", "ep_reduce.cu", "router.cu",
-           "norm.cu", "layer_few.cu")
+           "norm.cu", "layer_few.cu", "sample.cu")
 HEADERS = (CSRC / "common.cuh", INCLUDE / "b200moe.h")
 LIBRARY = PACKAGE_ROOT / "b200moe" / "libb200moe.so"
 GENCODE = "arch=compute_100a,code=sm_100a"

@@ -151,6 +151,11 @@ cudaError_t launch_layer_few(const void* x, const void* router, bool router_f32,
                              int experts, int top_k, double* logits, void* act_hi, void* act_lo,
                              void* out, int64_t* ids_out, float* weights_out, unsigned int* sync,
                              uint32_t* status, int sm_count, cudaStream_t stream);
+cudaError_t launch_sample(const void* logits, bool logits_f32, long long row_stride, int rows,
+                          int vocab, const float* uniforms, const float* temperature,
+                          float temperature_v, const int32_t* top_k, int top_k_v,
+                          const float* top_p, float top_p_v, const float* min_p, float min_p_v,
+                          int64_t* ids, float* logprobs, int sm_count, cudaStream_t stream);
 
 extern int g_gemm_stage_kb;
 extern int g_gemm_evict_first;
@@ -727,7 +732,8 @@ const char* b200moe_error_string(int code) {
     case B200MOE_E_LIMIT:
       return "the call exceeds a fixed limit of this entry point (b200moe_routing_static: "
              "4096 assignments; b200moe_ep_combine_reduce with B200MOE_FLAG_EP_PUSH: a grid "
-             "that is resident at once; b200moe_layer: 8 tokens, H <= 8192, I <= 65536)";
+             "that is resident at once; b200moe_layer: 8 tokens, H <= 8192, I <= 65536; "
+             "b200moe_sample: 2^20 rows, 2^18 tokens)";
     default: break;
   }
   if (code > 0) return cudaGetErrorString((cudaError_t)code);
@@ -882,6 +888,24 @@ int b200moe_add_rms_norm(const void* hidden, const void* residual, int residual_
   return (int)launch_add_rms_norm(hidden, residual, residual_is_f32 != 0, weight,
                                   weight_is_f32 != 0, rows, hidden_size, eps, out_bf16, codes_out,
                                   scale_out, residual_out, static_cast<cudaStream_t>(stream));
+}
+
+int b200moe_sample(const void* logits, int logits_are_f32, long long row_stride, int rows,
+                   int vocab, const float* uniforms, const float* temperature,
+                   float temperature_value, const int32_t* top_k, int top_k_value,
+                   const float* top_p, float top_p_value, const float* min_p, float min_p_value,
+                   int64_t* ids_out, float* logprobs_out, void* stream) {
+  if (!logits || !uniforms || !ids_out) return B200MOE_E_NULL;
+  if (rows < 1 || vocab < 1 || row_stride < vocab) return B200MOE_E_SHAPE;
+  if (rows > B200MOE_SAMPLE_MAX_ROWS || vocab > B200MOE_SAMPLE_MAX_VOCAB) return B200MOE_E_LIMIT;
+  if (reinterpret_cast<uintptr_t>(logits) % (logits_are_f32 ? 4 : 2)) return B200MOE_E_ALIGN;
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc) return rc;
+  return (int)launch_sample(logits, logits_are_f32 != 0, row_stride, rows, vocab, uniforms,
+                            temperature, temperature_value, top_k, top_k_value, top_p,
+                            top_p_value, min_p, min_p_value, ids_out, logprobs_out, dev.sm_count,
+                            static_cast<cudaStream_t>(stream));
 }
 
 int b200moe_tune(int knob, int value) {

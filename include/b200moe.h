@@ -513,6 +513,32 @@ int b200moe_layer(const B200MoeArgs* args, const void* router_weight, int router
                   int64_t* indices_out, float* weights_out, void* stream);
 
 /*
+ * One token per row of logits, from given random numbers (the step behind the model's head), one
+ * kernel.  No counterpart in the reference.  With w_i = exp((x_i - max) / temperature) and the
+ * order "larger logit first, lower id first among equal ones": min_p drops tokens with
+ * w_i < min_p, top_k keeps the first k of the order, top_p of those the shortest run of the order
+ * with at least top_p of their sum; the result is the first token i in id order for which the
+ * sum of the kept w up to i exceeds u times the sum of all kept.  NaN counts as -inf; tokens at
+ * -inf are never drawn; a row without any other token gives id -1 (log-probability -inf).
+ *   logits        [rows, vocab] bf16, or fp32 when logits_are_f32 != 0; row_stride elements
+ *                 from one row to the next, no alignment beyond the element's
+ *   uniforms      [rows] fp32 in [0, 1); 1 and more draw the last kept token, NaN the first
+ *   temperature, top_k, top_p, min_p   [rows] on the device, or NULL: the value behind it for
+ *                 every row.  Not above 0 / NaN: temperature takes the first of the order
+ *                 (log-probability 0), top_k is off, top_p keeps one token (NaN: off), min_p is
+ *                 off.  top_p >= 1 is off; min_p above 1 counts as 1.
+ *   ids_out       [rows] int64 out
+ *   logprobs_out  [rows] fp32 out or NULL: log of the probability that the token was drawn with
+ */
+#define B200MOE_SAMPLE_MAX_ROWS  1048576
+#define B200MOE_SAMPLE_MAX_VOCAB 262144
+int b200moe_sample(const void* logits, int logits_are_f32, long long row_stride, int rows,
+                   int vocab, const float* uniforms, const float* temperature,
+                   float temperature_value, const int32_t* top_k, int top_k_value,
+                   const float* top_p, float top_p_value, const float* min_p, float min_p_value,
+                   int64_t* ids_out, float* logprobs_out, void* stream);
+
+/*
  * Residual addition and root-mean-square norm of token rows (the step in front of the layer),
  * one kernel.  No counterpart in the reference.  Per row: s = hidden + residual in FP32,
  * residual_out = s in the residual's type, y = s * weight / sqrt(mean(s^2) + eps).
