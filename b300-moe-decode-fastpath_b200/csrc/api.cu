@@ -148,9 +148,10 @@ cudaError_t launch_add_rms_norm(const void* x, const void* residual, bool residu
 cudaError_t launch_layer_few(const void* x, const void* router, bool router_f32,
                              const void* gate_up, const void* down, const float* gate_up_scale,
                              const float* down_scale, int tokens, int hidden, int inter,
-                             int experts, int top_k, double* logits, void* act_hi, void* act_lo,
-                             void* out, int64_t* ids_out, float* weights_out, unsigned int* sync,
-                             uint32_t* status, int sm_count, cudaStream_t stream);
+                             int experts, int top_k, double* logits, uint32_t* act_max,
+                             void* act_hi, void* act_lo, void* out, int64_t* ids_out,
+                             float* weights_out, unsigned int* sync, uint32_t* status,
+                             int sm_count, cudaStream_t stream);
 cudaError_t launch_sample(const void* logits, bool logits_f32, long long row_stride, int rows,
                           int vocab, const float* uniforms, const float* temperature,
                           float temperature_v, const int32_t* top_k, int top_k_v,
@@ -862,7 +863,8 @@ int b200moe_layer(const B200MoeArgs* a, const void* router_weight, int router_is
       a->hidden_states, router_weight, router_is_f32 != 0, a->gate_up_weight, a->down_weight,
       fp8 ? a->gate_up_scale : nullptr, fp8 ? a->down_scale : nullptr, a->num_tokens,
       a->hidden_size, a->intermediate_size, a->num_experts, a->top_k,
-      reinterpret_cast<double*>(base + l.few_logits), a->swiglu_output, base + l.act_lo, a->output,
+      reinterpret_cast<double*>(base + l.few_logits),
+      reinterpret_cast<uint32_t*>(base + l.few_amax), a->swiglu_output, base + l.act_lo, a->output,
       indices_out, weights_out, reinterpret_cast<unsigned int*>(base + kFewSyncOffsetBytes),
       reinterpret_cast<uint32_t*>(base + l.status), c.dev.sm_count, c.stream);
 }

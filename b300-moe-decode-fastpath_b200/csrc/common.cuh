@@ -134,7 +134,8 @@ struct ScratchLayout {
   size_t x_scale;    // fp32 [rows_cap]
   size_t a_scale;    // fp32 [rows_cap]
   size_t a_amax;     // uint32 [rows_cap]  bit pattern of max |activation| per row
-  size_t few_logits; // fp64 [kFewMaxTokens, experts]  b200moe_layer only
+  size_t few_logits; // b200moe_layer only: fp64 [kFewMaxTokens, experts],
+  size_t few_amax;   //   uint32 [8 * kFewMaxTokens]  bit pattern of max |activation| per row
   size_t total;
 };
 
@@ -164,8 +165,9 @@ __host__ __device__ inline ScratchLayout scratch_layout(int rows_cap, int expert
   l.a_scale = align_up(l.x_scale + (size_t)rows_cap * sizeof(float), kScratchAlign);
   l.a_amax = align_up(l.a_scale + (size_t)rows_cap * sizeof(float), kScratchAlign);
   l.few_logits = align_up(l.a_amax + (size_t)rows_cap * sizeof(uint32_t), kScratchAlign);
-  l.total = align_up(l.few_logits + (size_t)kFewMaxTokens * experts * sizeof(double),
-                     kScratchAlign);
+  l.few_amax = align_up(l.few_logits + (size_t)kFewMaxTokens * experts * sizeof(double),
+                        kScratchAlign);
+  l.total = align_up(l.few_amax + 8 * kFewMaxTokens * sizeof(uint32_t), kScratchAlign);
   return l;
 }
 

@@ -13,21 +13,21 @@
 // Split.  Rows of the weight matrices are dealt out evenly to the blocks: block b takes
 // gate/up column pairs [b P / G, (b+1) P / G) of the P = (experts in use) * I pairs, and output
 // rows [b H / G, (b+1) H / G) of the down projection, for which it adds up all experts itself --
-// no partial sums in memory, no atomics, and sums in an order that only the shape and the
-// routing decide.  Inside the block the reduction dimension is cut into units of 128 bytes a
+// no partial sums in memory, no atomics on them, and sums in an order that only the shape and
+// the routing decide.  Inside the block the reduction dimension is cut into units of 128 bytes a
 // row, dealt to the warps in turn; the warps' partial tiles are added in shared memory.
 //
-// The tile.  A warp multiplies 16 rows by 8 columns with mma.m16n8k16.  The column index is the
-// token, for gate/up and down alike, so the token operand needs no gathering: for gate+up all
-// tokens are multiplied and only those routed to the expert are kept; for down the other tokens'
-// columns are zero and are masked once more when an expert's tile is added (a weight of NaN or
-// infinity reaches only the tokens routed to it).  mma.sync and not tcgen05: 8 columns of useful
-// work leave the tensor pipe idle either way, and operands that arrive in registers need no
-// descriptor, no tensor memory and no block-wide handshake per tile.
+// The tile.  A warp multiplies 16 or 32 rows by 8 columns with mma.m16n8k16.  The column index
+// is the token, for gate/up and down alike, so the token operand needs no gathering: for gate+up
+// all tokens are multiplied and only those routed to the expert are kept; for down the other
+// tokens' columns are zero and are masked once more when a unit's tile is added (a weight of NaN
+// or infinity reaches only the tokens routed to it).  mma.sync and not tcgen05: 8 columns of
+// useful work leave the tensor pipe idle either way, and operands that arrive in registers need
+// no descriptor, no tensor memory and no block-wide handshake per tile.
 //
 // Loads.  Each lane copies with cp.async the very 16 bytes that it will use as fragments (rows
 // g and g+8, four lanes side by side in a row), into a ring of its warp in shared memory, and
-// reads them back itself: no barrier between producer and consumer, and up to 200 KB in flight
+// reads them back itself: no barrier between producer and consumer, and up to 192 KB in flight
 // on an SM.  Any permutation of the reduction dimension is allowed as long as both operands
 // share it, which is why a lane's 16 consecutive bytes can serve as its part of the fragment.
 // The ring does not stop at the grid barrier: while a block waits for the activations, its
@@ -35,8 +35,15 @@
 //
 // Precision.  Logits are summed with the rounding errors of all additions kept (two-sum), so
 // that they are good to about 2^-48: experts that lie next to one another at the border are
-// told apart as in 64 bits.  Products and sums are FP32; the activations are held as the sum of
-// two BF16 numbers (16 significant bits), as the regular path holds them.
+// told apart as in 64 bits.  Products and sums are FP32.  With BF16 weights the activations are
+// held as the sum of two BF16 numbers (16 significant bits), as the regular path holds them.
+// With E4M3 weights both operands of the MMAs are FP16: one conversion instruction turns two
+// codes into two FP16 numbers exactly (to BF16 it takes five), token rows are multiplied by a
+// power of two that brings their largest element to [2^13, 2^14) and fit exactly, and
+// activations, scaled the same way, keep 11 significant bits (the regular path: twelve), which
+// is eight times finer than the BF16 rounding of the result.
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 
 namespace b200moe {
@@ -45,9 +52,8 @@ namespace {
 
 constexpr int kFewWarps = 16;
 constexpr int kFewThreads = kFewWarps * 32;
-constexpr int kFewStageBytes = 2048;            // 16 rows x 128 bytes: one stage of one warp
-constexpr int kFewSlots = kFewMaxTokens * 8;    // experts in use, at most
-constexpr int kFewMaxTiles = 4;                 // 16-row tiles of the down projection taken together
+constexpr int kFewSlots = kFewMaxTokens * 8;  // experts in use, at most; also assignments
+constexpr int kFewMaxTiles = 2;               // down tiles that share one load of the activations
 
 struct FewParams {
   const __nv_bfloat16* x;
@@ -58,10 +64,10 @@ struct FewParams {
   const float* down_scale;
   int tokens, hidden, inter, experts, top_k;
   int x_pitch;              // bytes of a token row in shared memory
-  int stages;               // ring stages of a warp
   double* logits;           // [tokens, experts]
-  __nv_bfloat16* act_hi;    // [tokens * top_k, inter]
-  __nv_bfloat16* act_lo;
+  uint32_t* act_max;        // [tokens * top_k]  E4M3 only: bit pattern of max |activation|
+  uint16_t* act_hi;         // [tokens * top_k, inter]  BF16 high parts; E4M3: FP32 bits 31..16
+  uint16_t* act_lo;         // BF16 low parts; E4M3: FP32 bits 15..0
   __nv_bfloat16* out;
   int64_t* ids_out;
   float* weights_out;
@@ -69,20 +75,29 @@ struct FewParams {
   uint32_t* status;
 };
 
+template <int SUBS>
 struct alignas(128) FewShared {
+  float red[kFewWarps][SUBS * 128];
   double logit[kFewWarps][kFewMaxTokens];
-  float red[2][kFewWarps][128];
   float weight[kFewSlots];              // by assignment
   int expert[kFewSlots];                // by slot (experts in use, ascending)
   int chosen[kFewSlots];                // expert by assignment
+  uint32_t act_max[kFewSlots];          // by assignment, of this block's activations
   int slot_of[B200MOE_MAX_EXPERTS];
   signed char assign[kFewSlots][kFewMaxTokens];  // assignment of (slot, token), or -1
+  uint8_t members[kFewSlots];           // tokens of a slot, one bit each
+  float x_unscale[kFewMaxTokens];       // E4M3: 2^-s of the token rows
+  float a_scale[kFewSlots];             // E4M3: 2^s of the activation rows
+  uint32_t x_max[kFewMaxTokens];
   int num_slots;
   int abort;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  const int bytes = valid ? 16 : 0;  // 0: the 16 bytes are zeroed, nothing is read
+// 16 bytes, or with bytes == 0 a piece of zeros, for which nothing is read and `src` (which may
+// lie behind the end of its matrix) is replaced by an address inside
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes,
+                                           const void* inside) {
+  src = bytes ? src : inside;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
@@ -93,18 +108,6 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// all but the newest `pending` groups have arrived
-__device__ __forceinline__ void cp_async_wait_for(int pending) {
-  switch (pending) {
-    case 0: cp_async_wait<0>(); break;
-    case 1: cp_async_wait<1>(); break;
-    case 2: cp_async_wait<2>(); break;
-    case 3: cp_async_wait<3>(); break;
-    case 4: cp_async_wait<4>(); break;
-    case 5: cp_async_wait<5>(); break;
-    default: cp_async_wait<6>(); break;
-  }
-}
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -113,13 +116,30 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
                : "memory");
   return v;
 }
+template <bool F16>
 __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                             uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// four E4M3 codes -> two FP16 pairs, exactly
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t w, uint32_t& p01, uint32_t& p23) {
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "mov.b32 {lo, hi}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+      : "=r"(p01), "=r"(p23)
+      : "r"(w));
 }
 
 // One 16-byte piece of rows g and g+8 times the token operand of the same elements: 8 BF16
@@ -133,23 +153,28 @@ __device__ __forceinline__ void multiply_piece(float (&c)[4], const uint4& top, 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t t01, t23, u01, u23;
-      e4m3x4_to_bf16x4(t[i], t01, t23);
-      e4m3x4_to_bf16x4(u[i], u01, u23);
-      mma_16x8x16(c, t01, u01, t23, u23, b[2 * i], b[2 * i + 1]);
+      e4m3x4_to_f16x4(t[i], t01, t23);
+      e4m3x4_to_f16x4(u[i], u01, u23);
+      mma_16x8x16<true>(c, t01, u01, t23, u23, b[2 * i], b[2 * i + 1]);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      mma_16x8x16(c, t[2 * i], u[2 * i], t[2 * i + 1], u[2 * i + 1], b[2 * i], b[2 * i + 1]);
+      mma_16x8x16<false>(c, t[2 * i], u[2 * i], t[2 * i + 1], u[2 * i + 1], b[2 * i], b[2 * i + 1]);
   }
 }
 
-// Grid barrier: bounded, after which the block goes on to its end without further work.
-__device__ __forceinline__ bool grid_barrier(unsigned int* counter, uint32_t* status, int* abort) {
+// Grid barrier in two halves: arrive, then wait (bounded; after that the block goes on to its
+// end without further work).
+__device__ __forceinline__ void grid_arrive(unsigned int* counter) {
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
     atomicAdd(counter, 1u);
+  }
+}
+__device__ __forceinline__ bool grid_wait(unsigned int* counter, uint32_t* status, int* abort) {
+  if (threadIdx.x == 0) {
     const uint64_t t0 = global_timer_ns();
     uint32_t spins = 0;
     while (true) {
@@ -176,41 +201,73 @@ __device__ __forceinline__ void two_sum(float& s, float& e, float p) {
   s = t;
 }
 
-// 64-bit order of a double: larger values larger, NaN above every number
+// 64-bit order of a double: larger values larger, NaN above every number, nothing at 0
 __device__ __forceinline__ unsigned long long order_of(double v) {
   const unsigned long long bits = (unsigned long long)__double_as_longlong(v);
   if (v != v) return ~0ull;
-  const unsigned long long k = (bits >> 63) ? ~bits : (bits | 0x8000000000000000ull);
-  return k;
+  return (bits >> 63) ? ~bits : (bits | 0x8000000000000000ull);
 }
 
-// Logits of the experts b, b + G, ...; x is in shared memory.
+// The power of two that brings a row with the largest magnitude `bits` (an FP32 pattern) to
+// [2^13, 2^14): no finite element overflows FP16, and elements down to 2^-27 of the largest keep
+// the eight bits of BF16.  A row of zeros: 1.  A row with infinities or NaN: 2^-114, under which
+// its finite elements stay finite.
+__device__ __forceinline__ float row_scale(uint32_t bits) {
+  if (bits == 0u) return 1.0f;
+  const int e = (int)(bits >> 23);            // biased exponent, 255 for inf and NaN
+  int s = e == 255 ? -114 : 13 + 127 - e;
+  s = s > 126 ? 126 : s;                      // subnormal rows
+  return __uint_as_float((uint32_t)(s + 127) << 23);
+}
+
 template <bool ROUTER_F32>
-__device__ __forceinline__ void router_logits(const FewParams& p, FewShared& sh,
+struct RouterVec {  // eight router weights in flight
+  uint4 raw[ROUTER_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* router, size_t at) {
+    if constexpr (ROUTER_F32) {
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(router) + at);
+      raw[0] = __ldg(src);
+      raw[1] = __ldg(src + 1);
+    } else {
+      raw[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(router) + at));
+    }
+  }
+  __device__ __forceinline__ void get(float (&w)[8]) const {
+    if constexpr (ROUTER_F32) {
+      const uint32_t r[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w,
+                             raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = __uint_as_float(r[i]);
+    } else {
+      const uint32_t r[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[2 * i] = __uint_as_float(r[i] << 16);
+        w[2 * i + 1] = __uint_as_float(r[i] & 0xFFFF0000u);
+      }
+    }
+  }
+};
+
+// Logits of the experts b, b + G, ...; x arrives in shared memory by the copies that the caller
+// has under way, the first router vectors of the block are loaded meanwhile.
+template <bool ROUTER_F32, typename Shared>
+__device__ __forceinline__ void router_logits(const FewParams& p, Shared& sh,
                                               const uint8_t* x_rows) {
   const int vecs = p.hidden / 8;
+  RouterVec<ROUTER_F32> first;
+  const bool has_first = blockIdx.x < p.experts && threadIdx.x < vecs;
+  if (has_first) first.load(p.router, (size_t)blockIdx.x * p.hidden + 8 * threadIdx.x);
+  cp_async_wait<0>();
+  __syncthreads();
   for (int e = blockIdx.x; e < p.experts; e += gridDim.x) {
     float s[kFewMaxTokens], err[kFewMaxTokens];
 #pragma unroll
     for (int t = 0; t < kFewMaxTokens; ++t) s[t] = err[t] = 0.0f;
     for (int v = threadIdx.x; v < vecs; v += kFewThreads) {
+      if (e != blockIdx.x || v != threadIdx.x) first.load(p.router, (size_t)e * p.hidden + 8 * v);
       float w[8];
-      if constexpr (ROUTER_F32) {
-        const float4* src = reinterpret_cast<const float4*>(
-            static_cast<const float*>(p.router) + (size_t)e * p.hidden + 8 * v);
-        const float4 a = __ldg(src), b = __ldg(src + 1);
-        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-        w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-      } else {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(
-            static_cast<const __nv_bfloat16*>(p.router) + (size_t)e * p.hidden + 8 * v));
-        const uint32_t words[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[2 * i] = __uint_as_float(words[i] << 16);
-          w[2 * i + 1] = __uint_as_float(words[i] & 0xFFFF0000u);
-        }
-      }
+      first.get(w);
 #pragma unroll
       for (int t = 0; t < kFewMaxTokens; ++t) {
         if (t >= p.tokens) break;
@@ -240,6 +297,7 @@ __device__ __forceinline__ void router_logits(const FewParams& p, FewShared& sh,
     __syncthreads();
     if (threadIdx.x < p.tokens) {
       double d = 0.0;
+#pragma unroll
       for (int i = 0; i < kFewWarps; ++i) d += sh.logit[i][threadIdx.x];
       __stcg(p.logits + (size_t)threadIdx.x * p.experts + e, d);
     }
@@ -248,13 +306,10 @@ __device__ __forceinline__ void router_logits(const FewParams& p, FewShared& sh,
 }
 
 // Top-k and softmax of every token, one warp each, then the list of experts in use.  Every
-// block does this for itself from the logits.
-__device__ __forceinline__ void choose_experts(const FewParams& p, FewShared& sh) {
+// block does this for itself from the logits; slot_of and assign are -1, members 0.
+template <typename Shared>
+__device__ __forceinline__ void choose_experts(const FewParams& p, Shared& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < B200MOE_MAX_EXPERTS; i += kFewThreads) sh.slot_of[i] = -1;
-  for (int i = threadIdx.x; i < kFewSlots * kFewMaxTokens; i += kFewThreads)
-    (&sh.assign[0][0])[i] = -1;
-  __syncthreads();
   if (warp < p.tokens) {
     double v[8];
     unsigned long long key[8];  // 0: taken or absent
@@ -265,18 +320,19 @@ __device__ __forceinline__ void choose_experts(const FewParams& p, FewShared& sh
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) key[i] = lane + 32 * i < p.experts ? order_of(v[i]) : 0ull;
-    double top = 0.0;
-    float mine = 0.0f, denom = 0.0f;
+    double mine = 0.0;
     int my_id = 0;
     for (int k = 0; k < p.top_k; ++k) {
-      unsigned long long best = 0ull;
+      unsigned long long best = key[0];
       int best_i = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 1; i < 8; ++i) {
+        if (32 * i >= p.experts) break;
         if (key[i] > best) {
           best = key[i];
           best_i = i;
         }
+      }
       const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32));
       const bool in_hi = (unsigned)(best >> 32) == hi;
       const unsigned lo = __reduce_max_sync(0xffffffffu, in_hi ? (unsigned)best : 0u);
@@ -291,17 +347,19 @@ __device__ __forceinline__ void choose_experts(const FewParams& p, FewShared& sh
           key[i] = 0ull;
         }
       value = __shfl_sync(0xffffffffu, value, id & 31);
-      if (k == 0) top = value;
-      const float w = expf((float)(value - top));
-      denom += w;
       if (lane == k) {
-        mine = w;
+        mine = value;
         my_id = (int)id;
       }
     }
+    const double top = __shfl_sync(0xffffffffu, mine, 0);
+    float w = lane < p.top_k ? expf((float)(mine - top)) : 0.0f;
+    float denom = w;
+#pragma unroll
+    for (int m = 4; m > 0; m >>= 1) denom += __shfl_xor_sync(0xffffffffu, denom, m);
     if (lane < p.top_k) {
       const int a = warp * p.top_k + lane;
-      const float w = mine / denom;
+      w /= denom;
       sh.weight[a] = w;
       sh.chosen[a] = my_id;
       sh.slot_of[my_id] = 0;  // in use; numbered below
@@ -326,34 +384,42 @@ __device__ __forceinline__ void choose_experts(const FewParams& p, FewShared& sh
       count += __popc(votes);
     }
     if (lane == 0) sh.num_slots = count;
+    __syncwarp();
+    for (int a = lane; a < p.tokens * p.top_k; a += 32)
+      sh.assign[sh.slot_of[sh.chosen[a]]][a / p.top_k] = (signed char)a;
+    __syncwarp();
+    for (int slot = lane; slot < count; slot += 32) {
+      unsigned m = 0u;
+#pragma unroll
+      for (int t = 0; t < kFewMaxTokens; ++t) m |= sh.assign[slot][t] >= 0 ? 1u << t : 0u;
+      sh.members[slot] = (uint8_t)m;
+    }
   }
-  __syncthreads();
-  if (threadIdx.x < p.tokens * p.top_k)
-    sh.assign[sh.slot_of[sh.chosen[threadIdx.x]]][threadIdx.x / p.top_k] = (signed char)threadIdx.x;
   __syncthreads();
 }
 
-// The order in which a warp's ring is filled: first the gate/up tiles of its block, then the
-// down tiles.  Both sides of the ring -- the copies and the products -- walk it.
-template <bool FP8>
+// What one block does, and the order in which a warp's ring is filled: first the gate/up tiles,
+// then the down tiles.  Both sides of the ring -- the copies and the products -- walk it.
+template <bool FP8, int SUBS>
 struct FewWork {
-  static constexpr int kUnit = FP8 ? 128 : 64;   // elements of a row in one stage
+  static constexpr int kUnit = FP8 ? 128 : 64;   // elements of a row in one stage (128 bytes)
   static constexpr int kPiece = FP8 ? 16 : 8;    // elements in 16 bytes
   static constexpr int kElem = FP8 ? 1 : 2;      // bytes of an element
+  static constexpr int kStageBytes = SUBS * 2048;
 
   int pair0, pairs, tiles, height;               // gate/up: this block's pairs and tiles
   int row0, rows, down_tiles, down_height;       // down: its output rows
   int units_h, units_i, down_units;              // stages along H; along I; along all experts
 
   __device__ FewWork(const FewParams& p, int slots) {
-    const long long total = (long long)slots * p.inter;
+    const unsigned total = (unsigned)slots * p.inter;   // at most 2^22, times the grid < 2^32
     pair0 = (int)(total * blockIdx.x / gridDim.x);
-    pairs = (int)(total * (blockIdx.x + 1) / gridDim.x) - pair0;
-    tiles = (pairs + 7) / 8;
+    pairs = (int)(total * (blockIdx.x + 1u) / gridDim.x) - pair0;
+    tiles = (pairs + 8 * SUBS - 1) / (8 * SUBS);
     height = tiles ? (pairs + tiles - 1) / tiles : 0;
-    row0 = (int)((long long)p.hidden * blockIdx.x / gridDim.x);
-    rows = (int)((long long)p.hidden * (blockIdx.x + 1) / gridDim.x) - row0;
-    down_tiles = (rows + 15) / 16;
+    row0 = (int)((unsigned)p.hidden * blockIdx.x / gridDim.x);
+    rows = (int)((unsigned)p.hidden * (blockIdx.x + 1u) / gridDim.x) - row0;
+    down_tiles = (rows + 16 * SUBS - 1) / (16 * SUBS);
     down_height = down_tiles ? (rows + down_tiles - 1) / down_tiles : 0;
     units_h = (p.hidden + kUnit - 1) / kUnit;
     units_i = (p.inter + kUnit - 1) / kUnit;
@@ -362,211 +428,319 @@ struct FewWork {
 };
 
 // Fills the ring: one stage per call, in order.
-template <bool FP8>
+template <bool FP8, int SUBS, int STAGES, typename Shared>
 struct FewProducer {
-  using Work = FewWork<FP8>;
+  using Work = FewWork<FP8, SUBS>;
   const FewParams& p;
-  const FewShared& sh;
+  const Shared& sh;
   const Work& w;
-  uint32_t ring;       // this lane's place in the warp's first stage
+  uint32_t dst, ring_end;
+  const uint8_t* top[SUBS];    // gate/up: this lane's gate rows, first piece
+  const uint8_t* base;         // down: this lane's row g of the group's first tile, first piece
+  size_t up_bytes;             // gate row -> up row of the same column
+  int ok[SUBS];                // gate/up: 16 where the row exists, else 0
+  int full, tail0, tail1;      // copied bytes of the two pieces in the last unit of a row
   int warp, lane;
-  int stage = 0;       // next stage to fill
-  bool down = false;
-  int tile = 0;        // gate/up: tile; down: first tile of the group
-  int unit;            // unit within the tile (gate/up) or along all experts (down)
-  int sub = 0;         // down: tile within the group
-  const uint8_t* top = nullptr;     // gate/up: this lane's gate row and up row
-  const uint8_t* bottom = nullptr;
-  bool live = false;
+  int tile = 0;                // gate/up: tile; down: first tile of the group
+  int unit;                    // gate/up: unit of the tile; down: unit of the expert
+  int slot = 0, sub = 0;       // down: expert, tile within the group
+  bool down = false, done = false;
 
-  __device__ FewProducer(const FewParams& p_, const FewShared& sh_, const Work& w_, uint32_t ring_,
+  __device__ FewProducer(const FewParams& p_, const Shared& sh_, const Work& w_, uint32_t ring,
                          int warp_, int lane_)
-      : p(p_), sh(sh_), w(w_), ring(ring_), warp(warp_), lane(lane_), unit(warp_) {
-    enter_tile();
+      : p(p_), sh(sh_), w(w_), dst(ring), ring_end(ring + STAGES * Work::kStageBytes), warp(warp_),
+        lane(lane_), unit(warp_) {
+    up_bytes = (size_t)p.inter * p.hidden * Work::kElem;
+    set_tail(p.hidden, w.units_h);
+    enter_gate();
   }
-
-  // moves on to the next tile that has a unit for this warp
-  __device__ void enter_tile() {
-    while (!down && unit >= w.units_h) {
+  __device__ __forceinline__ void set_tail(int length, int units) {
+    const int k = (units - 1) * Work::kUnit + (lane & 3) * Work::kPiece;
+    tail0 = k < length ? 16 : 0;
+    tail1 = k + Work::kUnit / 2 < length ? 16 : 0;
+  }
+  // moves on to the next gate/up tile that has a unit for this warp
+  __device__ __forceinline__ void enter_gate() {
+    while (unit >= w.units_h && tile < w.tiles) {
       unit -= w.units_h;
       ++tile;
-      if (tile >= w.tiles) break;
     }
-    if (!down && tile >= w.tiles) {
+    if (tile >= w.tiles) {
       down = true;
       tile = 0;
-      sub = 0;
       unit = warp;
+      set_tail(p.inter, w.units_i);
+      done = w.down_tiles == 0;
+      enter_down();
       return;
     }
-    const int i = tile * w.height + (lane >> 2);
-    live = (lane >> 2) < w.height && i < w.pairs;
-    const int pair = w.pair0 + (live ? i : 0);
-    const int slot = pair / p.inter;
-    const size_t col = (size_t)(pair - slot * p.inter);
-    const size_t row_bytes = (size_t)p.hidden * Work::kElem;
-    top = p.gate_up + ((size_t)sh.expert[slot] * 2 * p.inter + col) * row_bytes;
-    bottom = top + (size_t)p.inter * row_bytes;
+#pragma unroll
+    for (int s = 0; s < SUBS; ++s) {
+      const int i = s * 8 + (lane >> 2), local = tile * w.height + i;
+      const bool live = i < w.height && local < w.pairs;
+      ok[s] = live ? 16 : 0;
+      const int pair = w.pair0 + (live ? local : 0);
+      const int sl = pair / p.inter;
+      const size_t row = (size_t)sh.expert[sl] * 2 * p.inter + (pair - sl * p.inter);
+      top[s] = p.gate_up + row * p.hidden * Work::kElem + (lane & 3) * 16;
+    }
   }
-
-  __device__ void next() {
-    const uint32_t dst = ring + stage * kFewStageBytes;
-    const int piece = (lane & 3) * Work::kPiece;
+  // moves on to the expert that holds this warp's next unit
+  __device__ __forceinline__ void enter_down() {
+    while (!done && unit >= w.units_i) {
+      unit -= w.units_i;
+      if (++slot == sh.num_slots) {
+        slot = 0;
+        unit = warp;
+        tile += kFewMaxTiles;
+        done = tile >= w.down_tiles;
+      }
+    }
+    if (done) return;
+    const size_t row = (size_t)sh.expert[slot] * p.hidden + w.row0 + tile * w.down_height + (lane >> 2);
+    base = p.down + row * p.inter * Work::kElem + (lane & 3) * 16;
+  }
+  __device__ __forceinline__ void next() {
     if (!down) {
-      const int k = unit * Work::kUnit + piece, k2 = k + Work::kUnit / 2;
-      const bool a = live && k < p.hidden, b = live && k2 < p.hidden;
-      cp_async16(dst, a ? top + (size_t)k * Work::kElem : p.gate_up, a);
-      cp_async16(dst + 512, b ? top + (size_t)k2 * Work::kElem : p.gate_up, b);
-      cp_async16(dst + 1024, a ? bottom + (size_t)k * Work::kElem : p.gate_up, a);
-      cp_async16(dst + 1536, b ? bottom + (size_t)k2 * Work::kElem : p.gate_up, b);
+      const bool last = unit == w.units_h - 1;
+      const int m0 = last ? tail0 : 16, m1 = last ? tail1 : 16;
+#pragma unroll
+      for (int s = 0; s < SUBS; ++s) {
+        if (s * 8 >= w.height) break;
+        const uint8_t* a = top[s] + unit * 128;
+        const uint8_t* b = a + up_bytes;
+        cp_async16(dst + s * 2048, a, ok[s] & m0, p.gate_up);
+        cp_async16(dst + s * 2048 + 512, a + 64, ok[s] & m1, p.gate_up);
+        cp_async16(dst + s * 2048 + 1024, b, ok[s] & m0, p.gate_up);
+        cp_async16(dst + s * 2048 + 1536, b + 64, ok[s] & m1, p.gate_up);
+      }
       unit += kFewWarps;
-      if (unit >= w.units_h) enter_tile();
-    } else if (tile < w.down_tiles && unit < w.down_units) {
-      const int slot = unit / w.units_i;
-      const int k = (unit - slot * w.units_i) * Work::kUnit + piece, k2 = k + Work::kUnit / 2;
-      const int i = lane >> 2, r = (tile + sub) * w.down_height + i;
-      const bool t = i < w.down_height && r < w.rows;
-      const bool u = i + 8 < w.down_height && r + 8 < w.rows;
-      const uint8_t* base =
-          p.down + (((size_t)sh.expert[slot] * p.hidden + w.row0 + r) * p.inter + k) * Work::kElem;
-      const uint8_t* base8 = base + (size_t)8 * p.inter * Work::kElem;
-      const bool a = k < p.inter, b = k2 < p.inter;
-      const int half = Work::kUnit / 2 * Work::kElem;
-      cp_async16(dst, t && a ? base : p.down, t && a);
-      cp_async16(dst + 512, t && b ? base + half : p.down, t && b);
-      cp_async16(dst + 1024, u && a ? base8 : p.down, u && a);
-      cp_async16(dst + 1536, u && b ? base8 + half : p.down, u && b);
-      const int group = min(kFewMaxTiles, w.down_tiles - tile);
-      if (++sub == group) {
+      if (unit >= w.units_h) enter_gate();
+    } else if (!done) {
+      const bool last = unit == w.units_i - 1;
+      const int m0 = last ? tail0 : 16, m1 = last ? tail1 : 16;
+      const size_t stride = (size_t)p.inter * Work::kElem;
+      const uint8_t* a = base + (size_t)(sub * w.down_height) * stride + unit * 128;
+#pragma unroll
+      for (int h = 0; h < 2 * SUBS; ++h) {
+        if (h * 8 >= w.down_height) break;
+        const int i = h * 8 + (lane >> 2);
+        const bool live = i < w.down_height && (tile + sub) * w.down_height + i < w.rows;
+        cp_async16(dst + h * 1024, a, live ? m0 : 0, p.down);
+        cp_async16(dst + h * 1024 + 512, a + 64, live ? m1 : 0, p.down);
+        a += 8 * stride;
+      }
+      if (++sub == kFewMaxTiles || tile + sub == w.down_tiles) {
         sub = 0;
         unit += kFewWarps;
-        if (unit >= w.down_units) {
-          unit = warp;
-          tile += group;
-        }
+        if (unit >= w.units_i) enter_down();
       }
     }
     cp_async_commit();  // an empty group when there is nothing left
-    if (++stage == p.stages) stage = 0;
+    dst += Work::kStageBytes;
+    if (dst == ring_end) dst -= STAGES * Work::kStageBytes;
   }
 };
 
-template <bool FP8, bool ROUTER_F32>
+template <bool FP8, bool ROUTER_F32, int SUBS, int STAGES>
 __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewParams p) {
-  using Work = FewWork<FP8>;
+  using Work = FewWork<FP8, SUBS>;
+  using Shared = FewShared<SUBS>;
+  constexpr int kWords = FP8 ? 16 : 8;  // 32-bit words of the token operand in one unit
   extern __shared__ __align__(128) uint8_t smem[];
-  FewShared& sh = *reinterpret_cast<FewShared*>(smem);
-  uint8_t* x_rows = smem + sizeof(FewShared);
-  uint8_t* rings = x_rows + align_up((size_t)p.tokens * p.x_pitch, 128);
+  Shared& sh = *reinterpret_cast<Shared*>(smem);
+  uint8_t* x_rows = smem + sizeof(Shared);
+  const uint32_t rings = smem_u32(x_rows) + (uint32_t)align_up((size_t)p.tokens * p.x_pitch, 128);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
 
-  if (threadIdx.x == 0) {
-    sh.abort = 0;
-    if (blockIdx.x == 0) *p.status = 0u;
-  }
   // token rows, zero up to the end of the last unit
   const int row_vecs = (p.hidden + Work::kUnit - 1) / Work::kUnit * Work::kUnit / 8;
   for (int t = 0; t < p.tokens; ++t)
-    for (int v = threadIdx.x; v < row_vecs; v += kFewThreads) {
-      uint4 q = make_uint4(0u, 0u, 0u, 0u);
-      if (8 * v < p.hidden)
-        q = *reinterpret_cast<const uint4*>(p.x + (size_t)t * p.hidden + 8 * v);
-      *reinterpret_cast<uint4*>(x_rows + t * p.x_pitch + 16 * v) = q;
-    }
-  __syncthreads();
+    for (int v = threadIdx.x; v < row_vecs; v += kFewThreads)
+      cp_async16(smem_u32(x_rows) + t * p.x_pitch + 16 * v, p.x + (size_t)t * p.hidden + 8 * v,
+                 8 * v < p.hidden ? 16 : 0, p.x);
+  cp_async_commit();
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) *p.status = 0u;
+    if (FP8 && threadIdx.x < kFewSlots) p.act_max[threadIdx.x] = 0u;
+  }
+  if (threadIdx.x == 0) sh.abort = 0;
+  if (threadIdx.x < kFewSlots) {
+    sh.act_max[threadIdx.x] = 0u;
+    sh.members[threadIdx.x] = 0;
+  }
+  if (threadIdx.x < kFewMaxTokens) sh.x_max[threadIdx.x] = 0u;
+  if (threadIdx.x < B200MOE_MAX_EXPERTS) sh.slot_of[threadIdx.x] = -1;
+  (&sh.assign[0][0])[threadIdx.x] = -1;
+  static_assert(kFewThreads == kFewSlots * kFewMaxTokens, "one entry per thread");
   router_logits<ROUTER_F32>(p, sh, x_rows);
-  bool ok = grid_barrier(p.sync, p.status, &sh.abort);
+  grid_arrive(p.sync);
+
+  if constexpr (FP8) {  // token rows to scaled FP16, in place, while the other blocks arrive
+    const int vecs = row_vecs;
+    for (int t = 0; t < p.tokens; ++t) {
+      uint32_t most = 0u;
+      for (int v = threadIdx.x; v < vecs; v += kFewThreads) {
+        const uint4 q = *reinterpret_cast<const uint4*>(x_rows + t * p.x_pitch + 16 * v);
+        const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = max(most, max(words[i] & 0x7FFFu, (words[i] >> 16) & 0x7FFFu));
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 0) atomicMax(&sh.x_max[t], most);
+    }
+    __syncthreads();
+    for (int t = 0; t < p.tokens; ++t) {
+      const float scale = row_scale(sh.x_max[t] << 16);
+      if (threadIdx.x == 0) sh.x_unscale[t] = 1.0f / scale;
+      for (int v = threadIdx.x; v < vecs; v += kFewThreads) {
+        uint4* at = reinterpret_cast<uint4*>(x_rows + t * p.x_pitch + 16 * v);
+        const uint4 q = *at;
+        uint32_t words[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __half2 h = __floats2half2_rn(__uint_as_float(words[i] << 16) * scale,
+                                              __uint_as_float(words[i] & 0xFFFF0000u) * scale);
+          words[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        *at = make_uint4(words[0], words[1], words[2], words[3]);
+      }
+    }
+  }
+  bool ok = grid_wait(p.sync, p.status, &sh.abort);
 
   if (ok) {
     choose_experts(p, sh);
     const Work w(p, sh.num_slots);
-    const uint32_t ring = smem_u32(rings) + warp * p.stages * kFewStageBytes + lane * 16;
-    FewProducer<FP8> producer(p, sh, w, ring, warp, lane);
-    for (int i = 0; i < p.stages; ++i) producer.next();
-    int stage = 0;
-    const uint32_t x_lane = smem_u32(x_rows) + g * p.x_pitch + t4 * Work::kPiece * 2;
-    int buffer = 0;
+    uint32_t src = rings + warp * STAGES * Work::kStageBytes + lane * 16;
+    const uint32_t ring_end = src + STAGES * Work::kStageBytes;
+    FewProducer<FP8, SUBS, STAGES, Shared> producer(p, sh, w, src, warp, lane);
+#pragma unroll 1
+    for (int i = 0; i < STAGES; ++i) producer.next();
 
     // ---- gate + up -----------------------------------------------------------------
+    const uint32_t x_lane = smem_u32(x_rows) + g * p.x_pitch + t4 * Work::kPiece * 2;
     int unit = warp;
+#pragma unroll 1
     for (int tile = 0; tile < w.tiles; ++tile) {
-      float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (; unit < w.units_h; unit += kFewWarps) {
-        // token operand: elements of both halves of the unit
-        uint32_t b[FP8 ? 16 : 8];
+      float c[SUBS][4];
 #pragma unroll
-        for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
+      for (int s = 0; s < SUBS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[s][i] = 0.0f;
+#pragma unroll 1
+      for (; unit < w.units_h; unit += kFewWarps) {
+        uint32_t b[kWords];  // token operand: elements of both halves of the unit
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) {
           uint4 q = make_uint4(0u, 0u, 0u, 0u);
           if (g < p.tokens)
             q = lds128(x_lane + unit * Work::kUnit * 2 +
                        (FP8 ? (i / 2) * Work::kUnit + (i % 2) * 16 : i * Work::kUnit));
           b[4 * i] = q.x; b[4 * i + 1] = q.y; b[4 * i + 2] = q.z; b[4 * i + 3] = q.w;
         }
-        cp_async_wait_for(p.stages - 1);
-        const uint32_t src = ring + stage * kFewStageBytes;
-        const uint4 a0 = lds128(src), a1 = lds128(src + 512);
-        const uint4 b0 = lds128(src + 1024), b1 = lds128(src + 1536);
+        cp_async_wait<STAGES - 1>();
+        uint4 a[SUBS][4];
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[s][i] = lds128(src + s * 2048 + i * 512);
         producer.next();
-        if (++stage == p.stages) stage = 0;
-        multiply_piece<FP8>(c, a0, b0, b);
-        multiply_piece<FP8>(c, a1, b1, b + (FP8 ? 8 : 4));
+        src += Work::kStageBytes;
+        if (src == ring_end) src -= STAGES * Work::kStageBytes;
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s) {
+          multiply_piece<FP8>(c[s], a[s][0], a[s][2], b);
+          multiply_piece<FP8>(c[s], a[s][1], a[s][3], b + kWords / 2);
+        }
       }
       unit -= w.units_h;
-      float* red = sh.red[buffer][warp];
-      *reinterpret_cast<float2*>(red + g * 8 + 2 * t4) = make_float2(c[0], c[1]);
-      *reinterpret_cast<float2*>(red + (g + 8) * 8 + 2 * t4) = make_float2(c[2], c[3]);
+      __syncthreads();  // the sums of the tile before are read
+      if (2 * t4 < p.tokens) {
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s) {
+          float* red = sh.red[warp] + s * 128 + 2 * t4;
+          *reinterpret_cast<float2*>(red + g * 8) = make_float2(c[s][0], c[s][1]);
+          *reinterpret_cast<float2*>(red + (g + 8) * 8) = make_float2(c[s][2], c[s][3]);
+        }
+      }
       __syncthreads();
-      if (warp == tile % kFewWarps) {  // this warp finishes the tile, the others go on
+      if (threadIdx.x < 64 * SUBS) {  // one column pair of one token each
+        const int i = threadIdx.x >> 3, tok = threadIdx.x & 7;
+        const int local = tile * w.height + i;
+        if (i < w.height && local < w.pairs && tok < p.tokens) {
+          const int pair = w.pair0 + local;
+          const int slot = pair / p.inter, col = pair - slot * p.inter;
+          const int a = sh.assign[slot][tok];
+          if (a >= 0) {
+            const int at = (i >> 3) * 128 + (i & 7) * 8 + tok;
+            float gate = 0.0f, up = 0.0f;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int o = lane + 32 * half, i = o >> 3, tok = o & 7;
-          const int local = tile * w.height + i;
-          if (i < w.height && local < w.pairs && tok < p.tokens) {
-            const int pair = w.pair0 + local;
-            const int slot = pair / p.inter, col = pair - slot * p.inter;
-            const int a = sh.assign[slot][tok];
-            if (a >= 0) {
-              float gate = 0.0f, up = 0.0f;
-#pragma unroll
-              for (int i2 = 0; i2 < kFewWarps; ++i2) {
-                gate += sh.red[buffer][i2][o];
-                up += sh.red[buffer][i2][o + 64];
-              }
-              if constexpr (FP8) {
-                const float* s = p.gate_up_scale + (size_t)sh.expert[slot] * 2 * p.inter + col;
-                gate *= __ldg(s);
-                up *= __ldg(s + p.inter);
-              }
-              const float act = gate / (1.0f + expf(-gate)) * up * sh.weight[a];
-              const __nv_bfloat16 hi = __float2bfloat16_rn(act);
-              const float rest = act - __bfloat162float(hi);
-              p.act_hi[(size_t)a * p.inter + col] = hi;
-              p.act_lo[(size_t)a * p.inter + col] =
-                  __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);
+            for (int i2 = 0; i2 < kFewWarps; ++i2) {
+              gate += sh.red[i2][at];
+              up += sh.red[i2][at + 64];
             }
+            if constexpr (FP8) {
+              const float* s = p.gate_up_scale + (size_t)sh.expert[slot] * 2 * p.inter + col;
+              gate *= __ldg(s) * sh.x_unscale[tok];
+              up *= __ldg(s + p.inter) * sh.x_unscale[tok];
+            }
+            const float act = gate / (1.0f + expf(-gate)) * up * sh.weight[a];
+            uint16_t hi, lo;
+            if constexpr (FP8) {
+              const uint32_t bits = __float_as_uint(act);
+              hi = (uint16_t)(bits >> 16);
+              lo = (uint16_t)bits;
+              atomicMax(&sh.act_max[a], bits & 0x7FFFFFFFu);
+            } else {
+              const __nv_bfloat16 high = __float2bfloat16_rn(act);
+              const float rest = act - __bfloat162float(high);
+              hi = __bfloat16_as_ushort(high);
+              lo = __bfloat16_as_ushort(__float2bfloat16_rn(isfinite(rest) ? rest : 0.0f));
+            }
+            p.act_hi[(size_t)a * p.inter + col] = hi;
+            p.act_lo[(size_t)a * p.inter + col] = lo;
           }
         }
       }
-      buffer ^= 1;
     }
-    ok = grid_barrier(p.sync + 1, p.status, &sh.abort);
+    if constexpr (FP8) {
+      __syncthreads();
+      if (threadIdx.x < p.tokens * p.top_k && sh.act_max[threadIdx.x])
+        atomicMax(p.act_max + threadIdx.x, sh.act_max[threadIdx.x]);
+    }
+    grid_arrive(p.sync + 1);
+    ok = grid_wait(p.sync + 1, p.status, &sh.abort);
+    if constexpr (FP8) {
+      if (threadIdx.x < p.tokens * p.top_k)
+        sh.a_scale[threadIdx.x] = row_scale(__ldcg(p.act_max + threadIdx.x));
+      __syncthreads();
+    }
 
     // ---- down ----------------------------------------------------------------------
+#pragma unroll 1
     for (int first = 0; ok && first < w.down_tiles; first += kFewMaxTiles) {
-      const int group = min(kFewMaxTiles, w.down_tiles - first);
-      float total[kFewMaxTiles][4];
+      float total[kFewMaxTiles][SUBS][4];
 #pragma unroll
       for (int r = 0; r < kFewMaxTiles; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) total[r][i] = 0.0f;
-      for (int unit = warp; unit < w.down_units; unit += kFewWarps) {
-        const int slot = unit / w.units_i;
-        const int k = (unit - slot * w.units_i) * Work::kUnit + t4 * Work::kPiece;
-        const int a = sh.assign[slot][g];
-        uint32_t hi[FP8 ? 16 : 8], lo[FP8 ? 16 : 8];
+        for (int s = 0; s < SUBS; ++s)
 #pragma unroll
-        for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
+          for (int i = 0; i < 4; ++i) total[r][s][i] = 0.0f;
+      int slot = 0, unit = warp;
+#pragma unroll 1
+      while (true) {
+        while (unit >= w.units_i && slot < sh.num_slots) {
+          unit -= w.units_i;
+          ++slot;
+        }
+        if (slot >= sh.num_slots) break;
+        const int k = unit * Work::kUnit + t4 * Work::kPiece;
+        const int a = sh.assign[slot][g];
+        uint32_t hi[kWords], lo[kWords];
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) {
           const int at = k + (FP8 ? (i / 2) * (Work::kUnit / 2) + (i % 2) * 8 : i * (Work::kUnit / 2));
           uint4 q = make_uint4(0u, 0u, 0u, 0u), q2 = q;
           if (a >= 0 && at < p.inter) {
@@ -577,57 +751,88 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
           lo[4 * i] = q2.x; lo[4 * i + 1] = q2.y; lo[4 * i + 2] = q2.z; lo[4 * i + 3] = q2.w;
         }
         // the tokens of this lane's two columns
-        const bool has0 = sh.assign[slot][2 * t4] >= 0, has1 = sh.assign[slot][2 * t4 + 1] >= 0;
+        const unsigned members = sh.members[slot] >> (2 * t4);
+        float u0 = 1.0f, u1 = 1.0f;
+        if constexpr (FP8) {
+          const float scale = a >= 0 ? sh.a_scale[a] : 1.0f;
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) {
+            const __half2 h =
+                __floats2half2_rn(__uint_as_float(__byte_perm(lo[i], hi[i], 0x5410)) * scale,
+                                  __uint_as_float(__byte_perm(lo[i], hi[i], 0x7632)) * scale);
+            hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          const int a0 = sh.assign[slot][2 * t4], a1 = sh.assign[slot][2 * t4 + 1];
+          if (a0 >= 0) u0 = 1.0f / sh.a_scale[a0];
+          if (a1 >= 0) u1 = 1.0f / sh.a_scale[a1];
+        }
 #pragma unroll
         for (int r = 0; r < kFewMaxTiles; ++r) {
-          if (r >= group) break;
-          float s0 = 1.0f, s1 = 1.0f;
-          if constexpr (FP8) {
-            const int row = (first + r) * w.down_height + g;
-            const float* s = p.down_scale + (size_t)sh.expert[slot] * p.hidden + w.row0 + row;
-            s0 = g < w.down_height && row < w.rows ? __ldg(s) : 0.0f;
-            s1 = g + 8 < w.down_height && row + 8 < w.rows ? __ldg(s + 8) : 0.0f;
-          }
-          cp_async_wait_for(p.stages - 1);
-          const uint32_t src = ring + stage * kFewStageBytes;
-          const uint4 a0 = lds128(src), a1 = lds128(src + 512);
-          const uint4 b0 = lds128(src + 1024), b1 = lds128(src + 1536);
+          if (first + r >= w.down_tiles) break;
+          cp_async_wait<STAGES - 1>();
+          uint4 q[SUBS][4];
+#pragma unroll
+          for (int s = 0; s < SUBS; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[s][i] = lds128(src + s * 2048 + i * 512);
           producer.next();
-          if (++stage == p.stages) stage = 0;
-          float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          multiply_piece<FP8>(c, a0, b0, hi);
-          multiply_piece<FP8>(c, a1, b1, hi + (FP8 ? 8 : 4));
-          multiply_piece<FP8>(c, a0, b0, lo);
-          multiply_piece<FP8>(c, a1, b1, lo + (FP8 ? 8 : 4));
-          if (has0) {
-            total[r][0] = fmaf(c[0], s0, total[r][0]);
-            total[r][2] = fmaf(c[2], s1, total[r][2]);
-          }
-          if (has1) {
-            total[r][1] = fmaf(c[1], s0, total[r][1]);
-            total[r][3] = fmaf(c[3], s1, total[r][3]);
+          src += Work::kStageBytes;
+          if (src == ring_end) src -= STAGES * Work::kStageBytes;
+#pragma unroll
+          for (int s = 0; s < SUBS; ++s) {
+            if (s * 16 >= w.down_height) break;
+            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            multiply_piece<FP8>(c, q[s][0], q[s][2], hi);
+            multiply_piece<FP8>(c, q[s][1], q[s][3], hi + kWords / 2);
+            if constexpr (FP8) {
+              const int i = s * 16 + g, row = (first + r) * w.down_height + i;
+              const float* sc = p.down_scale + (size_t)sh.expert[slot] * p.hidden + w.row0 + row;
+              const float s0 = i < w.down_height && row < w.rows ? __ldg(sc) : 0.0f;
+              const float s1 = i + 8 < w.down_height && row + 8 < w.rows ? __ldg(sc + 8) : 0.0f;
+              c[0] *= s0 * u0;
+              c[1] *= s0 * u1;
+              c[2] *= s1 * u0;
+              c[3] *= s1 * u1;
+            } else {
+              multiply_piece<FP8>(c, q[s][0], q[s][2], lo);
+              multiply_piece<FP8>(c, q[s][1], q[s][3], lo + kWords / 2);
+            }
+            if (members & 1u) {
+              total[r][s][0] += c[0];
+              total[r][s][2] += c[2];
+            }
+            if (members & 2u) {
+              total[r][s][1] += c[1];
+              total[r][s][3] += c[3];
+            }
           }
         }
+        unit += kFewWarps;
       }
 #pragma unroll
       for (int r = 0; r < kFewMaxTiles; ++r) {
-        if (r >= group) break;
-        float* red = sh.red[buffer][warp];
-        *reinterpret_cast<float2*>(red + g * 8 + 2 * t4) = make_float2(total[r][0], total[r][1]);
-        *reinterpret_cast<float2*>(red + (g + 8) * 8 + 2 * t4) =
-            make_float2(total[r][2], total[r][3]);
+        if (first + r >= w.down_tiles) break;
+        __syncthreads();  // the sums of the tile before are read
+        if (2 * t4 < p.tokens) {
+#pragma unroll
+          for (int s = 0; s < SUBS; ++s) {
+            float* red = sh.red[warp] + s * 128 + 2 * t4;
+            *reinterpret_cast<float2*>(red + g * 8) = make_float2(total[r][s][0], total[r][s][1]);
+            *reinterpret_cast<float2*>(red + (g + 8) * 8) =
+                make_float2(total[r][s][2], total[r][s][3]);
+          }
+        }
         __syncthreads();
-        if (threadIdx.x < 128) {
-          const int i = threadIdx.x & 15, tok = threadIdx.x >> 4;
+        if (threadIdx.x < SUBS * 128) {
+          const int i = threadIdx.x % (SUBS * 16), tok = threadIdx.x / (SUBS * 16);
           const int row = (first + r) * w.down_height + i;
           if (i < w.down_height && row < w.rows && tok < p.tokens) {
             float v = 0.0f;
 #pragma unroll
-            for (int i2 = 0; i2 < kFewWarps; ++i2) v += sh.red[buffer][i2][i * 8 + tok];
+            for (int i2 = 0; i2 < kFewWarps; ++i2) v += sh.red[i2][i * 8 + tok];
             p.out[(size_t)tok * p.hidden + w.row0 + row] = __float2bfloat16_rn(v);
           }
         }
-        buffer ^= 1;
       }
     }
     cp_async_wait<0>();
@@ -639,11 +844,34 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
   }
 }
 
-int few_pitch(int hidden, bool fp8) {
-  // row pitch of the token operand: 64 (BF16) or 16 (FP8) bytes over a multiple of 128, which
-  // keeps the eight lanes of a 128-byte shared-memory read on different banks
-  const int unit = fp8 ? 128 : 64;
-  return (hidden + unit - 1) / unit * unit * 2 + (fp8 ? 16 : 64);
+// Stage size and ring depth for a call whose token rows take `x_bytes` of shared memory: stages
+// of 32 rows (4 KB a warp) where two of them fit, because half as many loops, barriers and
+// token-operand loads go with a byte; of 16 rows where the token rows are longer.
+struct FewShape {
+  int subs, stages;
+  size_t bytes;
+};
+bool few_shape(size_t x_bytes, FewShape* shape) {
+  constexpr size_t kMost = 227 * 1024;
+  const FewShape options[4] = {{2, 3, 0}, {2, 2, 0}, {1, 3, 0}, {1, 2, 0}};
+  for (const FewShape& o : options) {
+    const size_t fixed = o.subs == 2 ? sizeof(FewShared<2>) : sizeof(FewShared<1>);
+    const size_t bytes = fixed + x_bytes + (size_t)o.stages * kFewWarps * o.subs * 2048;
+    if (bytes <= kMost) {
+      *shape = {o.subs, o.stages, bytes};
+      return true;
+    }
+  }
+  return false;
+}
+
+template <bool FP8, bool ROUTER_F32>
+const void* few_kernel(const FewShape& s) {
+  if (s.subs == 2)
+    return s.stages == 3 ? (const void*)layer_few_kernel<FP8, ROUTER_F32, 2, 3>
+                         : (const void*)layer_few_kernel<FP8, ROUTER_F32, 2, 2>;
+  return s.stages == 3 ? (const void*)layer_few_kernel<FP8, ROUTER_F32, 1, 3>
+                       : (const void*)layer_few_kernel<FP8, ROUTER_F32, 1, 2>;
 }
 
 }  // namespace
@@ -651,9 +879,10 @@ int few_pitch(int hidden, bool fp8) {
 cudaError_t launch_layer_few(const void* x, const void* router, bool router_f32,
                              const void* gate_up, const void* down, const float* gate_up_scale,
                              const float* down_scale, int tokens, int hidden, int inter,
-                             int experts, int top_k, double* logits, void* act_hi, void* act_lo,
-                             void* out, int64_t* ids_out, float* weights_out, unsigned int* sync,
-                             uint32_t* status, int sm_count, cudaStream_t stream) {
+                             int experts, int top_k, double* logits, uint32_t* act_max,
+                             void* act_hi, void* act_lo, void* out, int64_t* ids_out,
+                             float* weights_out, unsigned int* sync, uint32_t* status,
+                             int sm_count, cudaStream_t stream) {
   const bool fp8 = gate_up_scale != nullptr;
   FewParams p;
   p.x = static_cast<const __nv_bfloat16*>(x);
@@ -667,31 +896,30 @@ cudaError_t launch_layer_few(const void* x, const void* router, bool router_f32,
   p.inter = inter;
   p.experts = experts;
   p.top_k = top_k;
-  p.x_pitch = few_pitch(hidden, fp8);
+  // row pitch of the token operand: 64 (BF16) or 16 (E4M3) bytes over a multiple of 128, which
+  // keeps the eight lanes of a 128-byte shared-memory read on different banks
+  const int unit = fp8 ? 128 : 64;
+  p.x_pitch = (hidden + unit - 1) / unit * unit * 2 + (fp8 ? 16 : 64);
   p.logits = logits;
-  p.act_hi = static_cast<__nv_bfloat16*>(act_hi);
-  p.act_lo = static_cast<__nv_bfloat16*>(act_lo);
+  p.act_max = act_max;
+  p.act_hi = static_cast<uint16_t*>(act_hi);
+  p.act_lo = static_cast<uint16_t*>(act_lo);
   p.out = static_cast<__nv_bfloat16*>(out);
   p.ids_out = ids_out;
   p.weights_out = weights_out;
   p.sync = sync;
   p.status = status;
-  constexpr size_t kMost = 227 * 1024;
-  const size_t fixed = sizeof(FewShared) + align_up((size_t)tokens * p.x_pitch, 128);
-  int stages = (int)((kMost - fixed) / (kFewWarps * kFewStageBytes));
-  if (kMost < fixed || stages < 1) return cudaErrorInvalidValue;
-  p.stages = stages > 6 ? 6 : stages;
-  const size_t bytes = fixed + (size_t)p.stages * kFewWarps * kFewStageBytes;
-  const void* kernel =
-      fp8 ? (router_f32 ? (const void*)layer_few_kernel<true, true>
-                        : (const void*)layer_few_kernel<true, false>)
-          : (router_f32 ? (const void*)layer_few_kernel<false, true>
-                        : (const void*)layer_few_kernel<false, false>);
+  FewShape shape;
+  if (!few_shape(align_up((size_t)tokens * p.x_pitch, 128), &shape)) return cudaErrorInvalidValue;
+  const void* kernel = fp8 ? (router_f32 ? few_kernel<true, true>(shape)
+                                         : few_kernel<true, false>(shape))
+                           : (router_f32 ? few_kernel<false, true>(shape)
+                                         : few_kernel<false, false>(shape));
   cudaError_t err =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shape.bytes);
   if (err != cudaSuccess) return err;
   void* args[] = {&p};
-  return cudaLaunchCooperativeKernel(kernel, dim3(sm_count), dim3(kFewThreads), args, bytes,
+  return cudaLaunchCooperativeKernel(kernel, dim3(sm_count), dim3(kFewThreads), args, shape.bytes,
                                      stream);
 }
 

@@ -5,8 +5,10 @@ cuts each of the 17 aligned terms, it is off by at most 17 * 2^-23 of the sum of
 magnitudes.  A warp chains at most ceil(units / 16) * 4 (BF16) or * 8 (E4M3) of them (a unit is
 64 or 128 elements) and 16 partial sums follow: `chain` below, times the sum of the products'
 magnitudes, bounds a dot product.  silu changes by at most 1.1 times its argument.  Activations
-are held as two BF16 numbers (2^-16), the few FP32 operations on them add 2^-20.  The result is
-rounded to BF16 (2^-8).  The bound is propagated element by element.
+are held as two BF16 numbers (2^-16), with E4M3 weights as FP16 numbers scaled so that the
+largest of a row is at least 2^13 (2^-12, and 2^-25 / 2^13 of the largest for those that become
+subnormal; the token rows, eight bits, only have the latter); the few FP32 operations on them
+add 2^-20.  The result is rounded to BF16 (2^-8).  The bound is propagated element by element.
 """
 
 from __future__ import annotations
@@ -57,11 +59,15 @@ def _formula(x, gate_up, down, ids, weights, fp8=False):
         eh, ei = _chain(gu.shape[1], fp8), _chain(inter, fp8, used)
         for t, k in (ids == e).nonzero().tolist():
             both, size = gu @ x[t], gu.abs() @ x[t].abs()
+            if fp8:
+                size = size + gu.abs().sum(-1) * x[t].abs().max() * 2.0 ** -38 / eh
             gate, up = both[:inter], both[inter:]
             silu, p = gate * torch.sigmoid(gate), float(weights[t, k])
             act = p * silu * up
             off = p * eh * (1.1 * size[:inter] * (up.abs() + eh * size[inter:])
                             + silu.abs() * size[inter:]) + act.abs() * (2.0 ** -16 + 2.0 ** -20)
+            if fp8:
+                off = off + act.abs() * 2.0 ** -12 + act.abs().max() * 2.0 ** -38
             out[t] += dn @ act
             # high and low part are multiplied one after the other: two chains
             bound[t] += dn.abs() @ (off + 2 * ei * (act.abs() + off))
