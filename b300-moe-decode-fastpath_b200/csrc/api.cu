@@ -149,9 +149,9 @@ cudaError_t launch_layer_few(const void* x, const void* router, bool router_f32,
                              const void* gate_up, const void* down, const float* gate_up_scale,
                              const float* down_scale, int tokens, int hidden, int inter,
                              int experts, int top_k, double* logits, uint32_t* act_max,
-                             void* act_hi, void* act_lo, void* out, int64_t* ids_out,
-                             float* weights_out, unsigned int* sync, uint32_t* status,
-                             int sm_count, cudaStream_t stream);
+                             void* acts, void* out, int64_t* ids_out, float* weights_out,
+                             unsigned int* sync, uint32_t* status, int sm_count,
+                             cudaStream_t stream);
 cudaError_t launch_sample(const void* logits, bool logits_f32, long long row_stride, int rows,
                           int vocab, const float* uniforms, const float* temperature,
                           float temperature_v, const int32_t* top_k, int top_k_v,
@@ -840,7 +840,7 @@ int b200moe_fp8_dequantize_rows(const uint8_t* q, const float* scale, long long 
 int b200moe_layer(const B200MoeArgs* a, const void* router_weight, int router_is_f32,
                   int64_t* indices_out, float* weights_out, void* stream) {
   if (!a || !a->hidden_states || !router_weight || !a->gate_up_weight || !a->down_weight ||
-      !a->swiglu_output || !a->output)
+      !a->output)
     return B200MOE_E_NULL;
   if (a->flags & ~(uint32_t)(B200MOE_FLAG_PDL | B200MOE_FLAG_FP8_WEIGHTS))
     return B200MOE_E_UNSUPPORTED;
@@ -854,7 +854,7 @@ int b200moe_layer(const B200MoeArgs* a, const void* router_weight, int router_is
   if (fp8 && (!a->gate_up_scale || !a->down_scale)) return B200MOE_E_NULL;
   if (fp8 && (a->hidden_size % 16 || a->intermediate_size % 16)) return B200MOE_E_ALIGN;
   if (!aligned16(a->hidden_states) || !aligned16(router_weight) || !aligned16(a->gate_up_weight) ||
-      !aligned16(a->down_weight) || !aligned16(a->swiglu_output))
+      !aligned16(a->down_weight))
     return B200MOE_E_ALIGN;
   const ScratchLayout l =
       scratch_layout(a->rows_cap, a->num_experts, a->hidden_size, a->intermediate_size);
@@ -864,7 +864,7 @@ int b200moe_layer(const B200MoeArgs* a, const void* router_weight, int router_is
       fp8 ? a->gate_up_scale : nullptr, fp8 ? a->down_scale : nullptr, a->num_tokens,
       a->hidden_size, a->intermediate_size, a->num_experts, a->top_k,
       reinterpret_cast<double*>(base + l.few_logits),
-      reinterpret_cast<uint32_t*>(base + l.few_amax), a->swiglu_output, base + l.act_lo, a->output,
+      reinterpret_cast<uint32_t*>(base + l.few_amax), base + l.few_acts, a->output,
       indices_out, weights_out, reinterpret_cast<unsigned int*>(base + kFewSyncOffsetBytes),
       reinterpret_cast<uint32_t*>(base + l.status), c.dev.sm_count, c.stream);
 }

@@ -135,7 +135,8 @@ struct ScratchLayout {
   size_t a_scale;    // fp32 [rows_cap]
   size_t a_amax;     // uint32 [rows_cap]  bit pattern of max |activation| per row
   size_t few_logits; // b200moe_layer only: fp64 [kFewMaxTokens, experts],
-  size_t few_amax;   //   uint32 [8 * kFewMaxTokens]  bit pattern of max |activation| per row
+  size_t few_amax;   //   uint32 [8 * kFewMaxTokens]  bit pattern of max |activation| per row,
+  size_t few_acts;   //   4 bytes [min(rows_cap, 8 * kFewMaxTokens), I]  activations
   size_t total;
 };
 
@@ -167,7 +168,9 @@ __host__ __device__ inline ScratchLayout scratch_layout(int rows_cap, int expert
   l.few_logits = align_up(l.a_amax + (size_t)rows_cap * sizeof(uint32_t), kScratchAlign);
   l.few_amax = align_up(l.few_logits + (size_t)kFewMaxTokens * experts * sizeof(double),
                         kScratchAlign);
-  l.total = align_up(l.few_amax + 8 * kFewMaxTokens * sizeof(uint32_t), kScratchAlign);
+  l.few_acts = align_up(l.few_amax + 8 * kFewMaxTokens * sizeof(uint32_t), kScratchAlign);
+  const int few_rows = rows_cap < 8 * kFewMaxTokens ? rows_cap : 8 * kFewMaxTokens;
+  l.total = align_up(l.few_acts + (size_t)few_rows * inter * 4, kScratchAlign);
   return l;
 }
 

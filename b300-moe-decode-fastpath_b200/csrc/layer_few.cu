@@ -64,6 +64,7 @@ struct FewParams {
   const float* down_scale;
   int tokens, hidden, inter, experts, top_k;
   int x_pitch;              // bytes of a token row in shared memory
+  unsigned long long inter_inverse;  // ceil(2^40 / inter)
   double* logits;           // [tokens, experts]
   uint32_t* act_max;        // [tokens * top_k]  E4M3 only: bit pattern of max |activation|
   uint16_t* act_hi;         // [tokens * top_k, inter]  BF16 high parts; E4M3: FP32 bits 31..16
@@ -78,18 +79,17 @@ struct FewParams {
 template <int SUBS>
 struct alignas(128) FewShared {
   float red[kFewWarps][SUBS * 128];
-  double logit[kFewWarps][kFewMaxTokens];
+  double logit[kFewWarps];
   float weight[kFewSlots];              // by assignment
   int expert[kFewSlots];                // by slot (experts in use, ascending)
   int chosen[kFewSlots];                // expert by assignment
   uint32_t act_max[kFewSlots];          // by assignment, of this block's activations
-  int slot_of[B200MOE_MAX_EXPERTS];
+  uint32_t used[B200MOE_MAX_EXPERTS / 32];  // experts in use, one bit each
   signed char assign[kFewSlots][kFewMaxTokens];  // assignment of (slot, token), or -1
-  uint8_t members[kFewSlots];           // tokens of a slot, one bit each
+  uint32_t members[kFewSlots];          // tokens of a slot, one bit each
   float x_unscale[kFewMaxTokens];       // E4M3: 2^-s of the token rows
   float a_scale[kFewSlots];             // E4M3: 2^s of the activation rows
   uint32_t x_max[kFewMaxTokens];
-  int num_slots;
   int abort;
 };
 
@@ -164,14 +164,11 @@ __device__ __forceinline__ void multiply_piece(float (&c)[4], const uint4& top, 
   }
 }
 
-// Grid barrier in two halves: arrive, then wait (bounded; after that the block goes on to its
-// end without further work).
+// Grid barrier in two halves: arrive (one thread, for the stores that come before it), then wait
+// (the block; bounded, after that it goes on to its end without further work).
 __device__ __forceinline__ void grid_arrive(unsigned int* counter) {
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    atomicAdd(counter, 1u);
-  }
+  asm volatile("fence.acq_rel.gpu;" ::: "memory");
+  asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
 }
 __device__ __forceinline__ bool grid_wait(unsigned int* counter, uint32_t* status, int* abort) {
   if (threadIdx.x == 0) {
@@ -201,11 +198,16 @@ __device__ __forceinline__ void two_sum(float& s, float& e, float p) {
   s = t;
 }
 
-// 64-bit order of a double: larger values larger, NaN above every number, nothing at 0
+// Order as integers: larger values larger, NaN above every number, 0 and -0 equal, nothing at 0
 __device__ __forceinline__ unsigned long long order_of(double v) {
-  const unsigned long long bits = (unsigned long long)__double_as_longlong(v);
+  const unsigned long long bits = (unsigned long long)__double_as_longlong(v + 0.0);
   if (v != v) return ~0ull;
   return (bits >> 63) ? ~bits : (bits | 0x8000000000000000ull);
+}
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t bits = __float_as_uint(v + 0.0f);
+  if (v != v) return ~0u;
+  return (bits >> 31) ? ~bits : (bits | 0x80000000u);
 }
 
 // The power of two that brings a row with the largest magnitude `bits` (an FP32 pattern) to
@@ -249,153 +251,157 @@ struct RouterVec {  // eight router weights in flight
   }
 };
 
-// Logits of the experts b, b + G, ...; x arrives in shared memory by the copies that the caller
-// has under way, the first router vectors of the block are loaded meanwhile.
+// Logits of the experts b, b + G, ...  Warps are dealt to (token, slice of the row): with T
+// tokens rounded up to a power of two P, warp w takes token w mod P and slice w / P of 16 / P.
+// x arrives in shared memory by copies that the caller has under way; each lane's first router
+// vector is loaded meanwhile.
 template <bool ROUTER_F32, typename Shared>
 __device__ __forceinline__ void router_logits(const FewParams& p, Shared& sh,
                                               const uint8_t* x_rows) {
-  const int vecs = p.hidden / 8;
-  RouterVec<ROUTER_F32> first;
-  const bool has_first = blockIdx.x < p.experts && threadIdx.x < vecs;
-  if (has_first) first.load(p.router, (size_t)blockIdx.x * p.hidden + 8 * threadIdx.x);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int shift = p.tokens > 4 ? 3 : p.tokens > 2 ? 2 : p.tokens > 1 ? 1 : 0;
+  const int token = warp & ((1 << shift) - 1), slices = kFewWarps >> shift;
+  const int vecs = p.hidden / 8, from = (warp >> shift) * 32 + lane;
+  const bool busy = token < p.tokens;
+  const uint8_t* x = x_rows + token * p.x_pitch;
+  RouterVec<ROUTER_F32> vec;
+  if (busy && blockIdx.x < p.experts && from < vecs)
+    vec.load(p.router, (size_t)blockIdx.x * p.hidden + 8 * from);
   cp_async_wait<0>();
   __syncthreads();
+#pragma unroll 1
   for (int e = blockIdx.x; e < p.experts; e += gridDim.x) {
-    float s[kFewMaxTokens], err[kFewMaxTokens];
-#pragma unroll
-    for (int t = 0; t < kFewMaxTokens; ++t) s[t] = err[t] = 0.0f;
-    for (int v = threadIdx.x; v < vecs; v += kFewThreads) {
-      if (e != blockIdx.x || v != threadIdx.x) first.load(p.router, (size_t)e * p.hidden + 8 * v);
-      float w[8];
-      first.get(w);
-#pragma unroll
-      for (int t = 0; t < kFewMaxTokens; ++t) {
-        if (t >= p.tokens) break;
-        const uint4 q = *reinterpret_cast<const uint4*>(x_rows + t * p.x_pitch + 16 * v);
+    float s = 0.0f, err = 0.0f;
+    if (busy) {
+#pragma unroll 1
+      for (int v = from; v < vecs; v += 32 * slices) {
+        float w[8];
+        vec.get(w);
+        int ahead = v + 32 * slices, ahead_e = e;
+        if (ahead >= vecs) {
+          ahead = from;
+          ahead_e += gridDim.x;
+        }
+        if (ahead_e < p.experts) vec.load(p.router, (size_t)ahead_e * p.hidden + 8 * ahead);
+        const uint4 q = *reinterpret_cast<const uint4*>(x + 16 * v);
         const uint32_t words[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float xv = (i & 1) ? __uint_as_float(words[i / 2] & 0xFFFF0000u)
                                    : __uint_as_float(words[i / 2] << 16);
           const float prod = __fmul_rn(w[i], xv);  // exact for BF16 x BF16
-          if constexpr (ROUTER_F32) err[t] += __fmaf_rn(w[i], xv, -prod);
-          two_sum(s[t], err[t], prod);
+          if constexpr (ROUTER_F32) err += __fmaf_rn(w[i], xv, -prod);
+          two_sum(s, err, prod);
         }
       }
     }
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // an error term of an overflowed or NaN sum is NaN itself: the sum alone tells
+    double d = (double)s;
+    if (isfinite(s)) d += (double)err;
 #pragma unroll
-    for (int t = 0; t < kFewMaxTokens; ++t) {
-      if (t >= p.tokens) break;
-      // an error term of an overflowed or NaN sum is NaN itself: the sum alone tells
-      double d = (double)s[t];
-      if (isfinite(s[t])) d += (double)err[t];
-#pragma unroll
-      for (int m = 16; m > 0; m >>= 1) d += __shfl_xor_sync(0xffffffffu, d, m);
-      if (lane == 0) sh.logit[warp][t] = d;
-    }
+    for (int m = 16; m > 0; m >>= 1) d += __shfl_xor_sync(0xffffffffu, d, m);
+    if (lane == 0) sh.logit[warp] = d;
     __syncthreads();
-    if (threadIdx.x < p.tokens) {
-      double d = 0.0;
-#pragma unroll
-      for (int i = 0; i < kFewWarps; ++i) d += sh.logit[i][threadIdx.x];
+    if (threadIdx.x < p.tokens) {  // all in warp 0, which arrives at the barrier
+      d = 0.0;
+      for (int i = 0; i < slices; ++i) d += sh.logit[(i << shift) + threadIdx.x];
       __stcg(p.logits + (size_t)threadIdx.x * p.experts + e, d);
     }
-    __syncthreads();
+    if (e + gridDim.x < p.experts) __syncthreads();
   }
 }
 
-// Top-k and softmax of every token, one warp each, then the list of experts in use.  Every
-// block does this for itself from the logits; slot_of and assign are -1, members 0.
+// Top-k of every token, one warp each, then the list of experts in use.  Every block does this
+// for itself from the logits.  The candidates are compared as FP32, which rounds the 64-bit logits monotonically; only
+// where two are equal as FP32 do the 64 bits decide, and then the lower id.
 template <typename Shared>
 __device__ __forceinline__ void choose_experts(const FewParams& p, Shared& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp < p.tokens) {
     double v[8];
-    unsigned long long key[8];  // 0: taken or absent
+    uint32_t key[8];  // 0: taken or absent
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int e = lane + 32 * i;
       v[i] = e < p.experts ? __ldcg(p.logits + (size_t)warp * p.experts + e) : 0.0;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) key[i] = lane + 32 * i < p.experts ? order_of(v[i]) : 0ull;
-    double mine = 0.0;
-    int my_id = 0;
+    for (int i = 0; i < 8; ++i) key[i] = lane + 32 * i < p.experts ? order_of((float)v[i]) : 0u;
+#pragma unroll 1
     for (int k = 0; k < p.top_k; ++k) {
-      unsigned long long best = key[0];
-      int best_i = 0;
+      uint32_t best = key[0];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) {
-        if (32 * i >= p.experts) break;
-        if (key[i] > best) {
-          best = key[i];
-          best_i = i;
-        }
-      }
-      const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32));
-      const bool in_hi = (unsigned)(best >> 32) == hi;
-      const unsigned lo = __reduce_max_sync(0xffffffffu, in_hi ? (unsigned)best : 0u);
-      const bool in_both = in_hi && (unsigned)best == lo;
-      const unsigned id =
-          __reduce_min_sync(0xffffffffu, in_both ? (unsigned)(lane + 32 * best_i) : 0xffffffffu);
-      double value = 0.0;
+      for (int i = 1; i < 8; ++i) best = max(best, key[i]);
+      best = __reduce_max_sync(0xffffffffu, best);
+      int held = 0, at = 0;  // how many of this lane's keys are the best one, and the last of them
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if ((unsigned)(lane + 32 * i) == id) {
-          value = v[i];
-          key[i] = 0ull;
+        if (key[i] == best) {
+          ++held;
+          at = i;
         }
-      value = __shfl_sync(0xffffffffu, value, id & 31);
-      if (lane == k) {
-        mine = value;
-        my_id = (int)id;
-      }
-    }
-    const double top = __shfl_sync(0xffffffffu, mine, 0);
-    float w = lane < p.top_k ? expf((float)(mine - top)) : 0.0f;
-    float denom = w;
+      const unsigned holders = __ballot_sync(0xffffffffu, held != 0);
+      unsigned id;
+      if ((holders & (holders - 1u)) == 0u && !__any_sync(0xffffffffu, held > 1)) {
+        id = __shfl_sync(0xffffffffu, (unsigned)(lane + 32 * at), __ffs(holders) - 1);
+      } else {
+        unsigned long long most = 0ull;  // among the equal ones, by all 64 bits
 #pragma unroll
-    for (int m = 4; m > 0; m >>= 1) denom += __shfl_xor_sync(0xffffffffu, denom, m);
+        for (int i = 0; i < 8; ++i)
+          if (key[i] == best && order_of(v[i]) > most) {
+            most = order_of(v[i]);
+            at = i;
+          }
+        const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(most >> 32));
+        const bool in_hi = (unsigned)(most >> 32) == hi;
+        const unsigned lo = __reduce_max_sync(0xffffffffu, in_hi ? (unsigned)most : 0u);
+        const bool in_both = held && in_hi && (unsigned)most == lo;
+        id = __reduce_min_sync(0xffffffffu, in_both ? (unsigned)(lane + 32 * at) : 0xffffffffu);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if ((unsigned)(lane + 32 * i) == id) key[i] = 0u;
+      if (lane == k) sh.chosen[warp * p.top_k + k] = (int)id;
+    }
+    __syncwarp();
     if (lane < p.top_k) {
-      const int a = warp * p.top_k + lane;
-      w /= denom;
-      sh.weight[a] = w;
-      sh.chosen[a] = my_id;
-      sh.slot_of[my_id] = 0;  // in use; numbered below
-      if (blockIdx.x == 0) {
-        if (p.ids_out) p.ids_out[a] = my_id;
-        if (p.weights_out) p.weights_out[a] = w;
-      }
+      const int id = sh.chosen[warp * p.top_k + lane];
+      atomicOr(&sh.used[id >> 5], 1u << (id & 31));
     }
   }
   __syncthreads();
-  if (warp == 0) {
-    int count = 0;
-    for (int base = 0; base < p.experts; base += 32) {
-      const int e = base + lane;
-      const bool used = e < p.experts && sh.slot_of[e] == 0;
-      const unsigned votes = __ballot_sync(0xffffffffu, used);
-      if (used) {
-        const int slot = count + __popc(votes & ((1u << lane) - 1u));
-        sh.slot_of[e] = slot;
-        sh.expert[slot] = e;
-      }
-      count += __popc(votes);
-    }
-    if (lane == 0) sh.num_slots = count;
-    __syncwarp();
-    for (int a = lane; a < p.tokens * p.top_k; a += 32)
-      sh.assign[sh.slot_of[sh.chosen[a]]][a / p.top_k] = (signed char)a;
-    __syncwarp();
-    for (int slot = lane; slot < count; slot += 32) {
-      unsigned m = 0u;
+  if (threadIdx.x < p.tokens * p.top_k) {  // number the experts in use in ascending order
+    const int a = threadIdx.x, e = sh.chosen[a], t = a / p.top_k;
+    int slot = __popc(sh.used[e >> 5] & ((1u << (e & 31)) - 1u));
 #pragma unroll
-      for (int t = 0; t < kFewMaxTokens; ++t) m |= sh.assign[slot][t] >= 0 ? 1u << t : 0u;
-      sh.members[slot] = (uint8_t)m;
-    }
+    for (int i = 0; i < B200MOE_MAX_EXPERTS / 32; ++i)
+      if (i < e >> 5) slot += __popc(sh.used[i]);
+    sh.expert[slot] = e;
+    sh.assign[slot][t] = (signed char)a;
+    atomicOr(&sh.members[slot], 1u << t);
+    if (blockIdx.x == 0 && p.ids_out) p.ids_out[a] = e;
   }
   __syncthreads();
+}
+
+// Softmax over a token's chosen logits, in its warp.
+template <typename Shared>
+__device__ __forceinline__ void softmax_weights(const FewParams& p, Shared& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (warp >= p.tokens) return;
+  const int a = warp * p.top_k + lane;
+  double mine = 0.0;
+  if (lane < p.top_k) mine = __ldcg(p.logits + (size_t)warp * p.experts + sh.chosen[a]);
+  const double top = __shfl_sync(0xffffffffu, mine, 0);
+  float w = lane < p.top_k ? expf((float)(mine - top)) : 0.0f;
+  float sum = w;
+#pragma unroll
+  for (int m = 4; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+  if (lane < p.top_k) {
+    w /= sum;
+    sh.weight[a] = w;
+    if (blockIdx.x == 0 && p.weights_out) p.weights_out[a] = w;
+  }
 }
 
 // What one block does, and the order in which a warp's ring is filled: first the gate/up tiles,
@@ -407,23 +413,37 @@ struct FewWork {
   static constexpr int kElem = FP8 ? 1 : 2;      // bytes of an element
   static constexpr int kStageBytes = SUBS * 2048;
 
-  int pair0, pairs, tiles, height;               // gate/up: this block's pairs and tiles
-  int row0, rows, down_tiles, down_height;       // down: its output rows
-  int units_h, units_i, down_units;              // stages along H; along I; along all experts
+  int row0, rows, down_tiles, down_height;       // down: this block's output rows
+  int units_h, units_i;                          // stages along H; along I
+  bool wide;                                     // down: a stage is 16 rows by two units
+  int pair0, pairs, tiles, height;               // gate/up: this block's pairs, in equal tiles
+  int slots;                                     // experts in use
 
-  __device__ FewWork(const FewParams& p, int slots) {
+  // what the dimensions alone say
+  __device__ explicit FewWork(const FewParams& p) {
+    row0 = (int)((unsigned)p.hidden * blockIdx.x / gridDim.x);
+    rows = (int)((unsigned)p.hidden * (blockIdx.x + 1u) / gridDim.x) - row0;
+    down_tiles = (rows + 16 * SUBS - 1) / (16 * SUBS);
+    down_height = down_tiles ? (rows + down_tiles - 1) / down_tiles : 0;
+    wide = SUBS == 2 && down_height <= 16;
+    const int unit = wide ? 2 * kUnit : kUnit;
+    units_h = (p.hidden + kUnit - 1) / kUnit;
+    units_i = (p.inter + unit - 1) / unit;
+  }
+  // and what the routing adds; used: one bit per expert in use
+  __device__ void deal_pairs(const FewParams& p, const uint32_t* used) {
+    slots = 0;
+#pragma unroll
+    for (int i = 0; i < B200MOE_MAX_EXPERTS / 32; ++i) slots += __popc(used[i]);
     const unsigned total = (unsigned)slots * p.inter;   // at most 2^22, times the grid < 2^32
     pair0 = (int)(total * blockIdx.x / gridDim.x);
     pairs = (int)(total * (blockIdx.x + 1u) / gridDim.x) - pair0;
     tiles = (pairs + 8 * SUBS - 1) / (8 * SUBS);
     height = tiles ? (pairs + tiles - 1) / tiles : 0;
-    row0 = (int)((unsigned)p.hidden * blockIdx.x / gridDim.x);
-    rows = (int)((unsigned)p.hidden * (blockIdx.x + 1u) / gridDim.x) - row0;
-    down_tiles = (rows + 16 * SUBS - 1) / (16 * SUBS);
-    down_height = down_tiles ? (rows + down_tiles - 1) / down_tiles : 0;
-    units_h = (p.hidden + kUnit - 1) / kUnit;
-    units_i = (p.inter + kUnit - 1) / kUnit;
-    down_units = slots * units_i;
+  }
+  // the expert (by slot) of a gate/up pair: pair / inter, exact for pairs below 2^24
+  static __device__ __forceinline__ int slot_of(const FewParams& p, int pair) {
+    return (int)(((unsigned long long)(unsigned)pair * p.inter_inverse) >> 40);
   }
 };
 
@@ -439,7 +459,7 @@ struct FewProducer {
   const uint8_t* base;         // down: this lane's row g of the group's first tile, first piece
   size_t up_bytes;             // gate row -> up row of the same column
   int ok[SUBS];                // gate/up: 16 where the row exists, else 0
-  int full, tail0, tail1;      // copied bytes of the two pieces in the last unit of a row
+  unsigned tail;               // pieces that exist in the last unit of a row, one bit each
   int warp, lane;
   int tile = 0;                // gate/up: tile; down: first tile of the group
   int unit;                    // gate/up: unit of the tile; down: unit of the expert
@@ -451,13 +471,19 @@ struct FewProducer {
       : p(p_), sh(sh_), w(w_), dst(ring), ring_end(ring + STAGES * Work::kStageBytes), warp(warp_),
         lane(lane_), unit(warp_) {
     up_bytes = (size_t)p.inter * p.hidden * Work::kElem;
-    set_tail(p.hidden, w.units_h);
+    set_tail(p.hidden, w.units_h, 1);
     enter_gate();
   }
-  __device__ __forceinline__ void set_tail(int length, int units) {
-    const int k = (units - 1) * Work::kUnit + (lane & 3) * Work::kPiece;
-    tail0 = k < length ? 16 : 0;
-    tail1 = k + Work::kUnit / 2 < length ? 16 : 0;
+  // pieces 2 s and 2 s + 1 of a stage are those of sub-tile s, or, where a stage holds `units` =
+  // 2 units, of the unit s
+  __device__ __forceinline__ void set_tail(int length, int count, int units) {
+    tail = 0u;
+#pragma unroll
+    for (int i = 0; i < 2 * SUBS; ++i) {
+      const int k = (count - 1) * units * Work::kUnit + (lane & 3) * Work::kPiece +
+                    (i & 1) * (Work::kUnit / 2) + (units == 2 ? (i >> 1) * Work::kUnit : 0);
+      if (k < length) tail |= 1u << i;
+    }
   }
   // moves on to the next gate/up tile that has a unit for this warp
   __device__ __forceinline__ void enter_gate() {
@@ -469,7 +495,7 @@ struct FewProducer {
       down = true;
       tile = 0;
       unit = warp;
-      set_tail(p.inter, w.units_i);
+      set_tail(p.inter, w.units_i, w.wide ? 2 : 1);
       done = w.down_tiles == 0;
       enter_down();
       return;
@@ -480,7 +506,7 @@ struct FewProducer {
       const bool live = i < w.height && local < w.pairs;
       ok[s] = live ? 16 : 0;
       const int pair = w.pair0 + (live ? local : 0);
-      const int sl = pair / p.inter;
+      const int sl = Work::slot_of(p, pair);
       const size_t row = (size_t)sh.expert[sl] * 2 * p.inter + (pair - sl * p.inter);
       top[s] = p.gate_up + row * p.hidden * Work::kElem + (lane & 3) * 16;
     }
@@ -489,7 +515,7 @@ struct FewProducer {
   __device__ __forceinline__ void enter_down() {
     while (!done && unit >= w.units_i) {
       unit -= w.units_i;
-      if (++slot == sh.num_slots) {
+      if (++slot == w.slots) {
         slot = 0;
         unit = warp;
         tile += kFewMaxTiles;
@@ -500,35 +526,38 @@ struct FewProducer {
     const size_t row = (size_t)sh.expert[slot] * p.hidden + w.row0 + tile * w.down_height + (lane >> 2);
     base = p.down + row * p.inter * Work::kElem + (lane & 3) * 16;
   }
+  __device__ __forceinline__ void copy(uint32_t to, const uint8_t* from, bool piece0, bool piece1,
+                                       const uint8_t* inside) {
+    cp_async16(to, from, piece0 ? 16 : 0, inside);
+    cp_async16(to + 512, from + 64, piece1 ? 16 : 0, inside);
+  }
   __device__ __forceinline__ void next() {
     if (!down) {
-      const bool last = unit == w.units_h - 1;
-      const int m0 = last ? tail0 : 16, m1 = last ? tail1 : 16;
+      const unsigned m = unit == w.units_h - 1 ? tail : 3u;
 #pragma unroll
       for (int s = 0; s < SUBS; ++s) {
         if (s * 8 >= w.height) break;
         const uint8_t* a = top[s] + unit * 128;
-        const uint8_t* b = a + up_bytes;
-        cp_async16(dst + s * 2048, a, ok[s] & m0, p.gate_up);
-        cp_async16(dst + s * 2048 + 512, a + 64, ok[s] & m1, p.gate_up);
-        cp_async16(dst + s * 2048 + 1024, b, ok[s] & m0, p.gate_up);
-        cp_async16(dst + s * 2048 + 1536, b + 64, ok[s] & m1, p.gate_up);
+        copy(dst + s * 2048, a, ok[s] && (m & 1u), ok[s] && (m & 2u), p.gate_up);
+        copy(dst + s * 2048 + 1024, a + up_bytes, ok[s] && (m & 1u), ok[s] && (m & 2u), p.gate_up);
       }
       unit += kFewWarps;
       if (unit >= w.units_h) enter_gate();
     } else if (!done) {
-      const bool last = unit == w.units_i - 1;
-      const int m0 = last ? tail0 : 16, m1 = last ? tail1 : 16;
-      const size_t stride = (size_t)p.inter * Work::kElem;
-      const uint8_t* a = base + (size_t)(sub * w.down_height) * stride + unit * 128;
+      const unsigned m = unit == w.units_i - 1 ? tail : 15u;
+      const size_t stride8 = (size_t)p.inter * (8 * Work::kElem);
+      const int row = (tile + sub) * w.down_height + (lane >> 2);
+      const uint8_t* a = base + (size_t)(sub * w.down_height) * p.inter * Work::kElem +
+                         unit * (w.wide ? 256 : 128);
 #pragma unroll
-      for (int h = 0; h < 2 * SUBS; ++h) {
-        if (h * 8 >= w.down_height) break;
-        const int i = h * 8 + (lane >> 2);
-        const bool live = i < w.down_height && (tile + sub) * w.down_height + i < w.rows;
-        cp_async16(dst + h * 1024, a, live ? m0 : 0, p.down);
-        cp_async16(dst + h * 1024 + 512, a + 64, live ? m1 : 0, p.down);
-        a += 8 * stride;
+      for (int s = 0; s < SUBS; ++s) {
+        const int i = (w.wide ? 0 : s * 16) + (lane >> 2), r = row + (w.wide ? 0 : s * 16);
+        const bool live = i < w.down_height && r < w.rows;
+        const bool live8 = i + 8 < w.down_height && r + 8 < w.rows;
+        const bool m0 = m & (1u << (2 * s)), m1 = m & (2u << (2 * s));
+        copy(dst + s * 2048, a, live && m0, live && m1, p.down);
+        copy(dst + s * 2048 + 1024, a + stride8, live8 && m0, live8 && m1, p.down);
+        a += w.wide ? (size_t)128 : 2 * stride8;
       }
       if (++sub == kFewMaxTiles || tile + sub == w.down_tiles) {
         sub = 0;
@@ -570,15 +599,23 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
     sh.act_max[threadIdx.x] = 0u;
     sh.members[threadIdx.x] = 0;
   }
-  if (threadIdx.x < kFewMaxTokens) sh.x_max[threadIdx.x] = 0u;
-  if (threadIdx.x < B200MOE_MAX_EXPERTS) sh.slot_of[threadIdx.x] = -1;
+  if (threadIdx.x < kFewMaxTokens) {
+    sh.x_max[threadIdx.x] = 0u;
+    sh.used[threadIdx.x] = 0u;
+  }
+  static_assert(kFewMaxTokens == B200MOE_MAX_EXPERTS / 32, "one word per thread");
   (&sh.assign[0][0])[threadIdx.x] = -1;
   static_assert(kFewThreads == kFewSlots * kFewMaxTokens, "one entry per thread");
   router_logits<ROUTER_F32>(p, sh, x_rows);
-  grid_arrive(p.sync);
+  if (warp == 0) {  // the block's logits were stored by this warp
+    __syncwarp();
+    if (lane == 0) grid_arrive(p.sync);
+  }
+  Work w(p);
 
   if constexpr (FP8) {  // token rows to scaled FP16, in place, while the other blocks arrive
     const int vecs = row_vecs;
+    __syncthreads();
     for (int t = 0; t < p.tokens; ++t) {
       uint32_t most = 0u;
       for (int v = threadIdx.x; v < vecs; v += kFewThreads) {
@@ -612,12 +649,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
 
   if (ok) {
     choose_experts(p, sh);
-    const Work w(p, sh.num_slots);
+    w.deal_pairs(p, sh.used);
     uint32_t src = rings + warp * STAGES * Work::kStageBytes + lane * 16;
     const uint32_t ring_end = src + STAGES * Work::kStageBytes;
     FewProducer<FP8, SUBS, STAGES, Shared> producer(p, sh, w, src, warp, lane);
 #pragma unroll 1
     for (int i = 0; i < STAGES; ++i) producer.next();
+    softmax_weights(p, sh);
 
     // ---- gate + up -----------------------------------------------------------------
     const uint32_t x_lane = smem_u32(x_rows) + g * p.x_pitch + t4 * Work::kPiece * 2;
@@ -671,7 +709,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
         const int local = tile * w.height + i;
         if (i < w.height && local < w.pairs && tok < p.tokens) {
           const int pair = w.pair0 + local;
-          const int slot = pair / p.inter, col = pair - slot * p.inter;
+          const int slot = Work::slot_of(p, pair), col = pair - slot * p.inter;
           const int a = sh.assign[slot][tok];
           if (a >= 0) {
             const int at = (i >> 3) * 128 + (i & 7) * 8 + tok;
@@ -710,7 +748,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
       if (threadIdx.x < p.tokens * p.top_k && sh.act_max[threadIdx.x])
         atomicMax(p.act_max + threadIdx.x, sh.act_max[threadIdx.x]);
     }
-    grid_arrive(p.sync + 1);
+    __syncthreads();
+    if (threadIdx.x == 0) grid_arrive(p.sync + 1);
     ok = grid_wait(p.sync + 1, p.status, &sh.abort);
     if constexpr (FP8) {
       if (threadIdx.x < p.tokens * p.top_k)
@@ -731,37 +770,63 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
       int slot = 0, unit = warp;
 #pragma unroll 1
       while (true) {
-        while (unit >= w.units_i && slot < sh.num_slots) {
+        while (unit >= w.units_i && slot < w.slots) {
           unit -= w.units_i;
           ++slot;
         }
-        if (slot >= sh.num_slots) break;
-        const int k = unit * Work::kUnit + t4 * Work::kPiece;
+        if (slot >= w.slots) break;
         const int a = sh.assign[slot][g];
-        uint32_t hi[kWords], lo[kWords];
-#pragma unroll
-        for (int i = 0; i < kWords / 4; ++i) {
-          const int at = k + (FP8 ? (i / 2) * (Work::kUnit / 2) + (i % 2) * 8 : i * (Work::kUnit / 2));
-          uint4 q = make_uint4(0u, 0u, 0u, 0u), q2 = q;
-          if (a >= 0 && at < p.inter) {
-            q = __ldcg(reinterpret_cast<const uint4*>(p.act_hi + (size_t)a * p.inter + at));
-            q2 = __ldcg(reinterpret_cast<const uint4*>(p.act_lo + (size_t)a * p.inter + at));
-          }
-          hi[4 * i] = q.x; hi[4 * i + 1] = q.y; hi[4 * i + 2] = q.z; hi[4 * i + 3] = q.w;
-          lo[4 * i] = q2.x; lo[4 * i + 1] = q2.y; lo[4 * i + 2] = q2.z; lo[4 * i + 3] = q2.w;
-        }
         // the tokens of this lane's two columns
         const unsigned members = sh.members[slot] >> (2 * t4);
+        uint32_t hi[SUBS][kWords], lo[SUBS][kWords];
+        float row_scales[kFewMaxTiles][SUBS][2];
+        if constexpr (FP8) {
+#pragma unroll
+          for (int r = 0; r < kFewMaxTiles; ++r)
+#pragma unroll
+            for (int s = 0; s < SUBS; ++s) {
+              const int i = (w.wide ? 0 : s * 16) + g, row = (first + r) * w.down_height + i;
+              const float* sc = p.down_scale + (size_t)sh.expert[slot] * p.hidden + w.row0 + row;
+              row_scales[r][s][0] = i < w.down_height && row < w.rows ? __ldg(sc) : 0.0f;
+              row_scales[r][s][1] = i + 8 < w.down_height && row + 8 < w.rows ? __ldg(sc + 8) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s) {
+          if (s && !w.wide) {  // both sub-tiles are of the same unit
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+              hi[s][i] = hi[0][i];
+              lo[s][i] = lo[0][i];
+            }
+            break;
+          }
+          const int k = (w.wide ? 2 * unit + s : unit) * Work::kUnit + t4 * Work::kPiece;
+#pragma unroll
+          for (int i = 0; i < kWords / 4; ++i) {
+            const int at =
+                k + (FP8 ? (i / 2) * (Work::kUnit / 2) + (i % 2) * 8 : i * (Work::kUnit / 2));
+            uint4 q = make_uint4(0u, 0u, 0u, 0u), q2 = q;
+            if (a >= 0 && at < p.inter) {
+              q = __ldcg(reinterpret_cast<const uint4*>(p.act_hi + (size_t)a * p.inter + at));
+              q2 = __ldcg(reinterpret_cast<const uint4*>(p.act_lo + (size_t)a * p.inter + at));
+            }
+            hi[s][4 * i] = q.x; hi[s][4 * i + 1] = q.y; hi[s][4 * i + 2] = q.z; hi[s][4 * i + 3] = q.w;
+            lo[s][4 * i] = q2.x; lo[s][4 * i + 1] = q2.y; lo[s][4 * i + 2] = q2.z; lo[s][4 * i + 3] = q2.w;
+          }
+          if constexpr (FP8) {
+            const float scale = a >= 0 ? sh.a_scale[a] : 1.0f;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+              const __half2 h = __floats2half2_rn(
+                  __uint_as_float(__byte_perm(lo[s][i], hi[s][i], 0x5410)) * scale,
+                  __uint_as_float(__byte_perm(lo[s][i], hi[s][i], 0x7632)) * scale);
+              hi[s][i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+          }
+        }
         float u0 = 1.0f, u1 = 1.0f;
         if constexpr (FP8) {
-          const float scale = a >= 0 ? sh.a_scale[a] : 1.0f;
-#pragma unroll
-          for (int i = 0; i < kWords; ++i) {
-            const __half2 h =
-                __floats2half2_rn(__uint_as_float(__byte_perm(lo[i], hi[i], 0x5410)) * scale,
-                                  __uint_as_float(__byte_perm(lo[i], hi[i], 0x7632)) * scale);
-            hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-          }
           const int a0 = sh.assign[slot][2 * t4], a1 = sh.assign[slot][2 * t4 + 1];
           if (a0 >= 0) u0 = 1.0f / sh.a_scale[a0];
           if (a1 >= 0) u1 = 1.0f / sh.a_scale[a1];
@@ -780,22 +845,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
           if (src == ring_end) src -= STAGES * Work::kStageBytes;
 #pragma unroll
           for (int s = 0; s < SUBS; ++s) {
-            if (s * 16 >= w.down_height) break;
             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            multiply_piece<FP8>(c, q[s][0], q[s][2], hi);
-            multiply_piece<FP8>(c, q[s][1], q[s][3], hi + kWords / 2);
+            multiply_piece<FP8>(c, q[s][0], q[s][2], hi[s]);
+            multiply_piece<FP8>(c, q[s][1], q[s][3], hi[s] + kWords / 2);
             if constexpr (FP8) {
-              const int i = s * 16 + g, row = (first + r) * w.down_height + i;
-              const float* sc = p.down_scale + (size_t)sh.expert[slot] * p.hidden + w.row0 + row;
-              const float s0 = i < w.down_height && row < w.rows ? __ldg(sc) : 0.0f;
-              const float s1 = i + 8 < w.down_height && row + 8 < w.rows ? __ldg(sc + 8) : 0.0f;
-              c[0] *= s0 * u0;
-              c[1] *= s0 * u1;
-              c[2] *= s1 * u0;
-              c[3] *= s1 * u1;
+              c[0] *= row_scales[r][s][0] * u0;
+              c[1] *= row_scales[r][s][0] * u1;
+              c[2] *= row_scales[r][s][1] * u0;
+              c[3] *= row_scales[r][s][1] * u1;
             } else {
-              multiply_piece<FP8>(c, q[s][0], q[s][2], lo);
-              multiply_piece<FP8>(c, q[s][1], q[s][3], lo + kWords / 2);
+              multiply_piece<FP8>(c, q[s][0], q[s][2], lo[s]);
+              multiply_piece<FP8>(c, q[s][1], q[s][3], lo[s] + kWords / 2);
             }
             if (members & 1u) {
               total[r][s][0] += c[0];
@@ -808,6 +868,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
           }
         }
         unit += kFewWarps;
+      }
+      if (w.wide) {  // two units of the same 16 rows
+#pragma unroll
+        for (int i = 0; i < 4; ++i) total[0][0][i] += total[0][SUBS - 1][i];
       }
 #pragma unroll
       for (int r = 0; r < kFewMaxTiles; ++r) {
@@ -880,9 +944,9 @@ cudaError_t launch_layer_few(const void* x, const void* router, bool router_f32,
                              const void* gate_up, const void* down, const float* gate_up_scale,
                              const float* down_scale, int tokens, int hidden, int inter,
                              int experts, int top_k, double* logits, uint32_t* act_max,
-                             void* act_hi, void* act_lo, void* out, int64_t* ids_out,
-                             float* weights_out, unsigned int* sync, uint32_t* status,
-                             int sm_count, cudaStream_t stream) {
+                             void* acts, void* out, int64_t* ids_out, float* weights_out,
+                             unsigned int* sync, uint32_t* status, int sm_count,
+                             cudaStream_t stream) {
   const bool fp8 = gate_up_scale != nullptr;
   FewParams p;
   p.x = static_cast<const __nv_bfloat16*>(x);
@@ -899,11 +963,12 @@ cudaError_t launch_layer_few(const void* x, const void* router, bool router_f32,
   // row pitch of the token operand: 64 (BF16) or 16 (E4M3) bytes over a multiple of 128, which
   // keeps the eight lanes of a 128-byte shared-memory read on different banks
   const int unit = fp8 ? 128 : 64;
+  p.inter_inverse = ((1ull << 40) + inter - 1) / inter;
   p.x_pitch = (hidden + unit - 1) / unit * unit * 2 + (fp8 ? 16 : 64);
   p.logits = logits;
   p.act_max = act_max;
-  p.act_hi = static_cast<uint16_t*>(act_hi);
-  p.act_lo = static_cast<uint16_t*>(act_lo);
+  p.act_hi = static_cast<uint16_t*>(acts);
+  p.act_lo = p.act_hi + (size_t)tokens * top_k * inter;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.ids_out = ids_out;
   p.weights_out = weights_out;

@@ -497,7 +497,7 @@ int b200moe_router_topk(const void* logits, int logits_are_f32, int num_tokens, 
  * reference.  For T <= B200MOE_LAYER_MAX_TOKENS; b200moe_forward takes larger calls.
  *   args          hidden_states, gate_up_weight, down_weight (and the two row scales with
  *                 B200MOE_FLAG_FP8_WEIGHTS, then H and I divisible by 16), the dimensions,
- *                 rows_cap, swiglu_output, scratch, output; flags 0 or
+ *                 rows_cap, scratch, output; flags 0 or
  *                 B200MOE_FLAG_FP8_WEIGHTS, B200MOE_FLAG_PDL (no effect).  All on the device.
  *   router_weight [E,H] bf16, or fp32 when router_is_f32 != 0
  *   indices_out   [T,K] int64 out or NULL

@@ -127,7 +127,7 @@ def test_c_entry_checks_its_arguments() -> None:
         a = _lib.B200MoeArgs()
         values = dict(hidden_states=4096, gate_up_weight=4096, down_weight=4096, num_tokens=2,
                       top_k=2, num_experts=8, hidden_size=64, intermediate_size=64, rows_cap=4,
-                      swiglu_output=4096, output=4096, scratch=4096, scratch_bytes=1 << 30)
+                      output=4096, scratch=4096, scratch_bytes=1 << 30)
         values.update(fields)
         for name, value in values.items():
             setattr(a, name, value)
@@ -135,7 +135,7 @@ def test_c_entry_checks_its_arguments() -> None:
 
     assert fn(None, 4096, 0, None, None, None) == -1
     assert call(router=None) == call(hidden_states=None) == call(gate_up_weight=None) == -1
-    assert call(swiglu_output=None) == call(output=None) == -1
+    assert call(output=None) == -1
     assert call(flags=_lib.FLAG_NVFP4_WEIGHTS) == call(flags=_lib.FLAG_LOCAL_EXPERTS) == -7
     assert call(num_tokens=9, rows_cap=18) == call(hidden_size=8200) == -8
     assert call(intermediate_size=65544) == -8
