@@ -9,13 +9,22 @@
 // -inf, tokens at -inf are never drawn; a row of nothing else gives -1.
 //
 // No sorting.  What is kept is a prefix of the order, so it is described by its last element: a
-// threshold on the logit and the index of the last token kept among those equal to it.  The
-// threshold is found by selection: a histogram over 2048 bins linear in m - x (for top-k of
-// counts, for top-p of weights) finds the bin where the wanted sum is crossed, then three
-// histograms over the digits (11, 11 and 10 bits) of the logit's ordered bit pattern find the
-// value inside that bin.  A row is read from memory once and stays in the shared memory of a
-// cluster of up to eight blocks, which exchange histograms and sums as distributed shared
-// memory.
+// threshold on the logit and the index of the last token kept among those equal to it.  A
+// histogram over 2048 bins linear in m - x (for top-k of counts, for top-p of weights) finds the
+// bin in which the wanted sum is crossed; the few hundred tokens of that bin are collected in a
+// list and each is compared with all others of it.  Where top-k leaves few tokens altogether
+// they are collected instead, and one block does the rest.  A bin with more than 1024 tokens
+// (equal logits, a range far from that of the weights) is taken apart by three histograms over
+// the digits (11, 11 and 10 bits) of the logit's ordered bit pattern.  A row is read from memory
+// once and stays in the shared memory of a cluster of up to eight blocks, which exchange
+// histograms, lists and sums as distributed shared memory.
+//
+// What bounds it.  One to a few rows: the chain of load, four to five cluster barriers and two
+// passes over shared memory.  Many rows: the FP64 exponentials (14 instructions a token and
+// pass) and the histogram's atomics.  Shared-memory atomics of 64 bits are loops of
+// compare-and-swap (9,000 to 16,000 cycles for 16,384 tokens, 240,000 where they meet in four
+// bins), those of 32 bits are not (1,300 and 4,300), so a weight is added as three parts of 15
+// bits.
 //
 // Exact sums.  With a large vocabulary the borders between tokens lie closer together than FP32
 // sums resolve, and sums in another order would move them.  The weights are therefore integers,
@@ -57,31 +66,44 @@ struct SampleParams {
   float* logprobs;
 };
 
-// ascending order of this key = descending order of the logit (no NaN)
+// ascending order of this key = descending order of the logit (no NaN); and back
 __device__ __forceinline__ uint32_t descending_key(float x) {
   // -0 and 0 are equal logits: adding 0 makes one of them
   const uint32_t bits = __float_as_uint(x + 0.0f);
   return (bits & 0x80000000u) ? bits : ~(bits | 0x80000000u);
 }
+__device__ __forceinline__ float logit_of(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? key : ~key & 0x7FFFFFFFu);
+}
 
-struct Published {       // what a block shows the others of its cluster
-  u64 sum;
-  u64 found[4];          // a selection's result: {bin, sum before, sum in bin, count in bin}
-  float best;
-  int first;
+// Weights are added up in the histogram as three parts of 15 bits (the highest may be 2^15):
+// with at most 2^15 tokens in a block their sums stay within 32 bits.
+constexpr int kPartBits = 15;
+constexpr int kGroups = 64;            // groups of 32 bins
+constexpr int kList = 1024;            // tokens that are compared one by one
+
+struct Found {
+  int bin;      // -1: the whole histogram stays below what was asked for
+  u64 before;   // sum of the bins before it
+  u64 amount;   // its own
 };
 
-struct SampleShared {
-  u64 mass[kBins];
-  unsigned count[kBins];
-  u64 bin_mass[kBins];       // cluster totals of the bins this block owns
-  unsigned bin_count[kBins];
+struct alignas(16) SampleShared {
+  uint32_t part[3][kBins];     // counts: the first one only
+  uint2 list[kList];           // {key, index}; the cluster's in its first block
+  u64 group[kGroups];          // of this block
+  u64 group_total[kGroups];    // of the cluster
   double power[64];
   u64 warp_sum[kSampleWarps];
-  Published pub;
+  u64 sum;                     // what a block shows the others: sum, largest logit, an index
+  float best;
+  int first;
+  unsigned list_n[2];          // of the count stage and of the weight stage
+  Found found;
   float warp_best[kSampleWarps];
   int warp_first[kSampleWarps];
-  u64 total;
+  uint32_t kept_key;
+  int kept_last;
 };
 
 // FP32 -> FP64 by moving bits (zero and subnormal numbers come out within 2^-126, which is
@@ -151,152 +173,217 @@ __device__ __forceinline__ u64 warp_total(u64 v) {
   return v;
 }
 
-// Sum over the cluster of one value per warp (already in sh.warp_sum); sh.pub.sum keeps the
-// block's own share.
-__device__ u64 cluster_total(SampleShared& sh, cg::cluster_group& cluster) {
+// Sum over the block of one value per warp (already in sh.warp_sum).
+__device__ __forceinline__ u64 block_total(SampleShared& sh) {
   __syncthreads();
-  if (threadIdx.x == 0) {
-    u64 s = 0ull;
-    for (int i = 0; i < kSampleWarps; ++i) s += sh.warp_sum[i];
-    sh.pub.sum = s;
-  }
-  cluster.sync();
   u64 s = 0ull;
-  for (unsigned r = 0; r < cluster.num_blocks(); ++r) s += cluster.map_shared_rank(&sh.pub, r)->sum;
+#pragma unroll
+  for (int i = 0; i < kSampleWarps; ++i) s += sh.warp_sum[i];
   return s;
 }
-
-// The bin of the cluster's histogram in which the running sum reaches `need` (1 <= need <= the
-// histogram's sum): {bin, sum before it, its sum, its count}.  BY_MASS: sums of weights, else of
-// counts.  Each block adds up its share of the bins over the cluster, the one whose share holds
-// the crossing finds it.
-template <bool BY_MASS>
-__device__ void find_bin(SampleShared& sh, cg::cluster_group& cluster, u64 need, u64 (&found)[4]) {
-  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int share = kBins / blocks;
-  cluster.sync();  // every block's histogram is complete
-  u64 mine = 0ull;
-  for (int b = threadIdx.x; b < share; b += kSampleThreads) {
-    u64 m = 0ull;
-    unsigned c = 0u;
-    for (int r = 0; r < blocks; ++r) {
-      if (BY_MASS) m += cluster.map_shared_rank(sh.mass, r)[rank * share + b];
-      c += cluster.map_shared_rank(sh.count, r)[rank * share + b];
-    }
-    sh.bin_mass[b] = BY_MASS ? m : (u64)c;
-    sh.bin_count[b] = c;
-    mine += BY_MASS ? m : (u64)c;
-  }
-  mine = warp_total(mine);
-  if ((threadIdx.x & 31) == 0) sh.warp_sum[threadIdx.x >> 5] = mine;
-  cluster_total(sh, cluster);
-  u64 before = 0ull;
-  int owner = 0;
-  for (; owner < blocks - 1; ++owner) {
-    const u64 s = cluster.map_shared_rank(&sh.pub, owner)->sum;
-    if (before + s >= need) break;
-    before += s;
-  }
-  if (owner == rank && threadIdx.x < 32) {
-    // 32 lanes, consecutive bins each
-    const int lane = threadIdx.x, per = share / 32;
-    u64 s = 0ull;
-    for (int i = 0; i < per; ++i) s += sh.bin_mass[lane * per + i];
-    u64 upto = s;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const u64 o = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += o;
-    }
-    u64 run = before + upto - s;
-    if (run < need && before + upto >= need) {
-      for (int i = 0; i < per; ++i) {
-        const u64 m = sh.bin_mass[lane * per + i];
-        if (run + m >= need) {
-          sh.pub.found[0] = (u64)(rank * share + lane * per + i);
-          sh.pub.found[1] = run;
-          sh.pub.found[2] = m;
-          sh.pub.found[3] = sh.bin_count[lane * per + i];
-          break;
-        }
-        run += m;
-      }
-    }
-  }
+// The same over the cluster; sh.sum keeps the block's own share.
+__device__ __forceinline__ u64 cluster_total(SampleShared& sh, cg::cluster_group& cluster) {
+  const u64 mine = block_total(sh);
+  if (threadIdx.x == 0) sh.sum = mine;
   cluster.sync();
-  for (int i = 0; i < 4; ++i) found[i] = cluster.map_shared_rank(&sh.pub, owner)->found[i];
+  u64 s = 0ull;
+  for (unsigned r = 0; r < cluster.num_blocks(); ++r) s += *cluster.map_shared_rank(&sh.sum, r);
+  return s;
 }
 
 template <bool BY_MASS>
 __device__ __forceinline__ void clear_bins(SampleShared& sh) {
   for (int b = threadIdx.x; b < kBins; b += kSampleThreads) {
-    if (BY_MASS) sh.mass[b] = 0ull;
-    sh.count[b] = 0u;
+    sh.part[0][b] = 0u;
+    if (BY_MASS) sh.part[1][b] = sh.part[2][b] = 0u;
   }
 }
+__device__ __forceinline__ void add_mass(SampleShared& sh, int bin, u64 w) {
+  constexpr uint32_t mask = (1u << kPartBits) - 1u;
+  atomicAdd(&sh.part[0][bin], (uint32_t)w & mask);
+  atomicAdd(&sh.part[1][bin], (uint32_t)(w >> kPartBits) & mask);
+  atomicAdd(&sh.part[2][bin], (uint32_t)(w >> (2 * kPartBits)));
+}
+template <bool BY_MASS>
+__device__ __forceinline__ u64 bin_amount(const uint32_t (*part)[kBins], int bin) {
+  u64 v = part[0][bin];
+  if (BY_MASS) v += ((u64)part[1][bin] << kPartBits) + ((u64)part[2][bin] << (2 * kPartBits));
+  return v;
+}
+__device__ __forceinline__ u64 inclusive_scan(u64 v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const u64 o = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
 
-// The shortest prefix of the kept tokens whose sum (of counts, or of weights) reaches `need`;
-// the histogram over the linear bins is in sh.mass / sh.count.
+// The bin of the cluster's histogram in which the running sum reaches need(total), and the
+// histogram's total.  Every block finds it for itself: from the sums of 64 groups of 32 bins of
+// all blocks, then from the bins of one group.
+template <bool BY_MASS, typename Need>
+__device__ Found find_bin(SampleShared& sh, cg::cluster_group& cluster, Need need_of, u64& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int blocks = (int)cluster.num_blocks();
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kGroups / kSampleWarps; ++i) {
+    const int group = warp * (kGroups / kSampleWarps) + i;
+    const u64 v = warp_total(bin_amount<BY_MASS>(sh.part, group * 32 + lane));
+    if (lane == 0) sh.group[group] = v;
+  }
+  cluster.sync();
+  {  // as many neighbouring lanes as there are blocks share a group
+    static_assert(kGroups * kMaxCluster <= kSampleThreads, "one group of one block per thread");
+    const int group = threadIdx.x / blocks, r = threadIdx.x % blocks;
+    u64 v = group < kGroups ? cluster.map_shared_rank(sh.group, r)[group] : 0ull;
+    for (int m = blocks >> 1; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    if (group < kGroups && r == 0) sh.group_total[group] = v;
+  }
+  __syncthreads();
+  const u64 a = sh.group_total[2 * lane], b = sh.group_total[2 * lane + 1];
+  const u64 upto = inclusive_scan(a + b);
+  total = __shfl_sync(0xffffffffu, upto, 31);
+  const u64 need = need_of(total);
+  Found found;
+  found.bin = -1;
+  found.before = found.amount = 0ull;
+  if (need > total) return found;  // in every block alike
+  const int at = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;
+  u64 before = __shfl_sync(0xffffffffu, upto - a - b, at);
+  const u64 first = __shfl_sync(0xffffffffu, a, at);
+  int group = 2 * at;
+  if (before + first < need) {
+    before += first;
+    ++group;
+  }
+  if (warp == 0) {
+    const int bin = group * 32 + lane;
+    u64 v = 0ull;
+    for (int r = 0; r < blocks; ++r)
+      v += bin_amount<BY_MASS>(cluster.map_shared_rank(sh.part, r), bin);
+    const u64 run = before + inclusive_scan(v);
+    if (lane == __ffs(__ballot_sync(0xffffffffu, run >= need)) - 1) {
+      sh.found.bin = bin;
+      sh.found.before = run - v;
+      sh.found.amount = v;
+    }
+  }
+  __syncthreads();
+  return sh.found;
+}
+
+// Appends the warp's chosen tokens to the list of the cluster's first block; `count` goes on
+// counting where the list is full.
+__device__ __forceinline__ void append(bool chosen, uint32_t key, int index, uint2* list,
+                                       unsigned* count) {
+  const unsigned votes = __ballot_sync(0xffffffffu, chosen);
+  if (votes == 0u) return;
+  const int lane = threadIdx.x & 31, leader = __ffs(votes) - 1;
+  unsigned base = 0u;
+  if (lane == leader) base = atomicAdd(count, (unsigned)__popc(votes));
+  base = __shfl_sync(0xffffffffu, base, leader);
+  const unsigned at = base + __popc(votes & ((1u << lane) - 1u));
+  if (chosen && at < (unsigned)kList) list[at] = make_uint2(key, (unsigned)index);
+}
+__device__ __forceinline__ u64 place(const uint2& e) { return ((u64)e.x << 32) | e.y; }
+
+// The shortest prefix of the kept tokens whose sum (of counts, or of weights) ends in bin
+// `found.bin` of the linear histogram, `rest` (at least 1) into it.
 template <bool BY_MASS>
 __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& row,
-                       const Weigher& weigh, const Kept kept, u64 need) {
-  u64 found[4];
-  find_bin<BY_MASS>(sh, cluster, need, found);
-  const int bin = (int)found[0];
-  u64 rest = need - found[1];
+                       const Weigher& weigh, const Kept kept, const int bin, u64 rest) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int from = warp * row.chunk, to = min(row.n, from + row.chunk);
+  // the bin's tokens
+  uint2* list = cluster.map_shared_rank(sh.list, 0);
+  unsigned* count = cluster.map_shared_rank(&sh.list_n[BY_MASS], 0);
+  for (int i = from; i < to; i += 32) {
+    const float v = i + lane < to ? row.x[i + lane] : -INFINITY;
+    const uint32_t key = descending_key(v);
+    append(v != -INFINITY && row.bin(v) == bin && kept.holds(key, row.base + i + lane), key,
+           row.base + i + lane, list, count);
+  }
+  cluster.sync();
+  const unsigned n = *count;
+  Kept next;
+  if (n <= (unsigned)kList) {
+    // a copy of the list, with the weights behind it, where the histogram was
+    uint2* own = reinterpret_cast<uint2*>(&sh.part[0][0]);
+    u64* weight = reinterpret_cast<u64*>(&sh.part[1][0]);
+    static_assert(kList * sizeof(uint2) == sizeof(sh.part[0]) &&
+                      kList * sizeof(u64) == sizeof(sh.part[0]), "they fit");
+    for (unsigned i = threadIdx.x; i < n; i += kSampleThreads) {
+      own[i] = list[i];
+      weight[i] = BY_MASS ? weigh(logit_of(own[i].x)) : 1ull;
+    }
+    __syncthreads();
+    for (unsigned i = threadIdx.x; i < n; i += kSampleThreads) {
+      const u64 mine = place(own[i]);
+      u64 before = 0ull;
+#pragma unroll 4
+      for (unsigned j = 0; j < n; ++j) before += place(own[j]) < mine ? weight[j] : 0ull;
+      if (before < rest && before + weight[i] >= rest) {
+        sh.kept_key = own[i].x;
+        sh.kept_last = (int)own[i].y;
+      }
+    }
+    __syncthreads();
+    next.key = sh.kept_key;
+    next.last = sh.kept_last;
+    cluster.sync();  // the first block's list has been read
+    return next;
+  }
+
   uint32_t prefix = 0u, mask = 0u;
   const int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
+  Found found;
 #pragma unroll 1
   for (int level = 0; level < 3; ++level) {
     const int shift = shifts[level];
     const uint32_t digits = (1u << widths[level]) - 1u;
-    __syncthreads();
+    cluster.sync();  // the histogram before has been read
     clear_bins<BY_MASS>(sh);
     __syncthreads();
     for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
       const float v = row.x[i];
       const uint32_t key = descending_key(v);
       if (row.bin(v) != bin || (key & mask) != prefix || !kept.holds(key, row.base + i)) continue;
-      u64 w = 0ull;
-      if (BY_MASS) {
-        w = weigh(v);
-        if (w == 0ull) continue;
-        atomicAdd(&sh.mass[(key >> shift) & digits], w);
-      }
-      atomicAdd(&sh.count[(key >> shift) & digits], 1u);
+      const int digit = (key >> shift) & digits;
+      if (BY_MASS) add_mass(sh, digit, weigh(v));
+      else atomicAdd(&sh.part[0][digit], 1u);
     }
-    find_bin<BY_MASS>(sh, cluster, rest, found);
-    rest -= found[1];
-    prefix |= (uint32_t)found[0] << shift;
+    u64 total;
+    found = find_bin<BY_MASS>(sh, cluster, [&](u64) { return rest; }, total);
+    rest -= found.before;
+    prefix |= (uint32_t)found.bin << shift;
     mask |= digits << shift;
   }
   // all tokens of the last bin have the same logit: how many of them are needed
-  const u64 equal = found[3];
-  const u64 each = BY_MASS ? found[2] / equal : 1ull;
+  const u64 each = BY_MASS ? weigh(logit_of(prefix)) : 1ull;
+  const u64 equal = found.amount / each;
   const u64 ties = (rest + each - 1ull) / each;
-  Kept next;
   next.key = prefix;
   next.last = 0x7FFFFFFF;
   if (ties >= equal) {
     if (prefix == kept.key) next.last = kept.last;
+    cluster.sync();  // the histogram has been read
     return next;
   }
   // the index of the ties-th of them
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int from = warp * row.chunk, to = min(row.n, from + row.chunk);
-  unsigned n = 0u;
+  unsigned hits = 0u;
   for (int i = from + lane; i < to; i += 32)
-    n += descending_key(row.x[i]) == prefix && kept.holds(prefix, row.base + i);
-  n = __reduce_add_sync(0xffffffffu, n);
-  if (lane == 0) sh.warp_sum[warp] = n;
+    hits += descending_key(row.x[i]) == prefix && kept.holds(prefix, row.base + i);
+  hits = __reduce_add_sync(0xffffffffu, hits);
+  if (lane == 0) sh.warp_sum[warp] = hits;
+  if (threadIdx.x == 0) sh.first = -1;
   cluster_total(sh, cluster);
   u64 before = 0ull;
-  for (unsigned r = 0; r < cluster.block_rank(); ++r)
-    before += cluster.map_shared_rank(&sh.pub, r)->sum;
+  for (unsigned r = 0; r < cluster.block_rank(); ++r) before += *cluster.map_shared_rank(&sh.sum, r);
   for (int i = 0; i < warp; ++i) before += sh.warp_sum[i];
-  if (threadIdx.x == 0) sh.pub.first = -1;
-  __syncthreads();
-  if (before < ties && before + n >= ties) {  // in this warp's tokens
+  if (before < ties && before + hits >= ties) {  // in this warp's tokens
     for (int i = from; i < to; i += 32) {
       const bool hit = i + lane < to && descending_key(row.x[i + lane]) == prefix &&
                        kept.holds(prefix, row.base + i + lane);
@@ -304,7 +391,7 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
       const unsigned want = (unsigned)(ties - before);  // >= 1
       if ((unsigned)__popc(votes) >= want) {
         if (hit && (unsigned)__popc(votes & ((2u << lane) - 1u)) == want)
-          sh.pub.first = row.base + i + lane;
+          sh.first = row.base + i + lane;
         break;
       }
       before += __popc(votes);
@@ -312,34 +399,156 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
   }
   cluster.sync();
   for (unsigned r = 0; r < cluster.num_blocks(); ++r) {
-    const int f = cluster.map_shared_rank(&sh.pub, r)->first;
+    const int f = *cluster.map_shared_rank(&sh.first, r);
     if (f >= 0) next.last = f;
   }
   cluster.sync();
   return next;
 }
 
+// Top-p's share of a sum of weights, at least 1.
+__device__ __forceinline__ u64 mass_needed(float top_p, u64 total) {
+  const double need = ceil((double)fmaxf(top_p, 0.0f) * (double)total);
+  return need < 1.0 ? 1ull : (u64)need;
+}
+// The weight at which the draw falls.
+__device__ __forceinline__ u64 draw_target(float u, u64 total) {
+  const u64 target = u > 0.0f ? (u64)((double)fminf(u, 1.0f) * (double)total) : 0ull;
+  return target >= total ? total - 1ull : target;
+}
+__device__ __forceinline__ void store_result(const SampleParams& p, int row_id,
+                                             const Weigher& weigh, int index, float x, u64 total) {
+  p.ids[row_id] = index;
+  if (p.logprobs)
+    p.logprobs[row_id] = (float)(weigh.exponent(x) * 0.69314718055994530942 -
+                                 (log((double)total) - kWeightBits * 0.69314718055994530942));
+}
+
+// All that is left after top-k fits the list: one block cuts it to k tokens, weighs them, cuts to
+// top-p and draws, comparing every token with every other.
+__device__ void finish_list(SampleShared& sh, const SampleParams& p, int row_id,
+                            const Weigher& weigh, int top_k, float top_p, float u) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = (int)sh.list_n[0];
+  constexpr int kEach = kList / kSampleThreads;
+  u64* weight = reinterpret_cast<u64*>(&sh.part[0][0]);
+  for (int i = threadIdx.x; i < n; i += kSampleThreads) weight[i] = weigh(logit_of(sh.list[i].x));
+  __syncthreads();
+  u64 mine[kEach], before[kEach], sum = 0ull;
+#pragma unroll
+  for (int q = 0; q < kEach; ++q) {
+    const int i = threadIdx.x + q * kSampleThreads;
+    mine[q] = before[q] = 0ull;
+    if (i >= n) continue;
+    const u64 at = place(sh.list[i]);
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j)
+      if (place(sh.list[j]) < at) {
+        ++rank;
+        before[q] += weight[j];
+      }
+    if (rank < top_k) mine[q] = weight[i];
+    sum += mine[q];
+  }
+  sum = warp_total(sum);
+  if (lane == 0) sh.warp_sum[warp] = sum;
+  u64 total = block_total(sh);  // and all weights have been read
+  if (top_p < 1.0f) {
+    const u64 need = mass_needed(top_p, total);
+    __syncthreads();
+    sum = 0ull;
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      if (before[q] >= need) mine[q] = 0ull;
+      sum += mine[q];
+    }
+    sum = warp_total(sum);
+    if (lane == 0) sh.warp_sum[warp] = sum;
+    total = block_total(sh);
+  }
+#pragma unroll
+  for (int q = 0; q < kEach; ++q) {
+    const int i = threadIdx.x + q * kSampleThreads;
+    if (i < n) weight[i] = mine[q];
+  }
+  __syncthreads();
+  const u64 target = draw_target(u, total);
+#pragma unroll
+  for (int q = 0; q < kEach; ++q) {
+    if (mine[q] == 0ull) continue;
+    const uint2 e = sh.list[threadIdx.x + q * kSampleThreads];
+    u64 run = 0ull;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) run += sh.list[j].y < e.y ? weight[j] : 0ull;
+    if (run <= target && target < run + mine[q])
+      store_result(p, row_id, weigh, (int)e.y, logit_of(e.x), total);
+  }
+}
+
+// The block's logits into shared memory at x[0..n), NaN as -inf; returns the thread's largest.
+// 16-byte loads where the row's address allows, all of a thread's in flight at once.
+__device__ __forceinline__ float keep(float v, float& best) {
+  if (v != v) v = -INFINITY;
+  best = fmaxf(best, v);
+  return v;
+}
+// elements in front of the first 16-byte boundary
 template <typename T>
-__device__ __forceinline__ float logit_at(const T* p, int i);
-template <>
-__device__ __forceinline__ float logit_at<float>(const float* p, int i) { return __ldg(p + i); }
-template <>
-__device__ __forceinline__ float logit_at<__nv_bfloat16>(const __nv_bfloat16* p, int i) {
-  return __bfloat162float(p[i]);
+__device__ __forceinline__ int head_of(const T* src) {
+  return (int)((16u - (unsigned)(reinterpret_cast<uintptr_t>(src) & 15u)) % 16u / sizeof(T));
+}
+// x + head_of(src) is on a 16-byte boundary too
+template <typename T>
+__device__ __forceinline__ float load_row(const T* __restrict__ src, int n, float* x) {
+  constexpr int kVec = 16 / sizeof(T), kAhead = 8;
+  float best = -INFINITY;
+  const int head = min(n, head_of(src));
+  const int vecs = (n - head) / kVec;
+  for (int start = threadIdx.x; start < vecs; start += kAhead * kSampleThreads) {
+    uint4 q[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (start + i * kSampleThreads < vecs)
+        q[i] = __ldg(reinterpret_cast<const uint4*>(src + head) + start + i * kSampleThreads);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (start + i * kSampleThreads >= vecs) break;
+      float4* dst = reinterpret_cast<float4*>(x + head + (start + i * kSampleThreads) * kVec);
+      const uint32_t words[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+      float v[kVec];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) {
+          v[j] = keep(__uint_as_float(words[j]), best);
+        } else {
+          v[2 * j] = keep(__uint_as_float(words[j] << 16), best);
+          v[2 * j + 1] = keep(__uint_as_float(words[j] & 0xFFFF0000u), best);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kVec / 4; ++j)
+        dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    }
+  }
+  const int rest = n - vecs * kVec;  // before and behind the vectors
+  if (threadIdx.x < rest) {
+    const int i = threadIdx.x < head ? threadIdx.x : threadIdx.x + vecs * kVec;
+    x[i] = keep((float)src[i], best);
+  }
+  return best;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   SampleShared& sh = *reinterpret_cast<SampleShared*>(smem);
-  float* x = reinterpret_cast<float*>(smem + sizeof(SampleShared));
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), blocks = (int)cluster.num_blocks();
   const int row_id = blockIdx.x / blocks;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
   Row row;
-  row.x = x;
   row.base = min(p.vocab, rank * p.slice);
   row.n = min(p.vocab - row.base, p.slice);
   row.chunk = (row.n + 32 * kSampleWarps - 1) / (32 * kSampleWarps) * 32;
@@ -352,26 +561,23 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
 
   // the row's tokens into shared memory, and the largest
   const T* src = static_cast<const T*>(p.logits) + (size_t)row_id * p.row_stride + row.base;
-  float best = -INFINITY;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
-    float v = logit_at<T>(src, i);
-    if (v != v) v = -INFINITY;
-    x[i] = v;
-    best = fmaxf(best, v);
-  }
+  float* x = reinterpret_cast<float*>(smem + sizeof(SampleShared)) + ((4 - head_of(src)) & 3);
+  row.x = x;
+  clear_bins<true>(sh);
   if (threadIdx.x < 64) sh.power[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+  if (threadIdx.x < 2) sh.list_n[threadIdx.x] = 0u;
+  float best = load_row<T>(src, row.n, x);
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, m));
   if (lane == 0) sh.warp_best[warp] = best;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < kSampleWarps; ++i) best = fmaxf(best, sh.warp_best[i]);
-    sh.pub.best = best;
+    sh.best = best;
   }
   cluster.sync();
   best = -INFINITY;
-  for (int r = 0; r < blocks; ++r) best = fmaxf(best, cluster.map_shared_rank(&sh.pub, r)->best);
+  for (int r = 0; r < blocks; ++r) best = fmaxf(best, *cluster.map_shared_rank(&sh.best, r));
   row.best = best;
 
   if (best == -INFINITY || !(temperature > 0.0f)) {  // nothing to draw, or nothing to draw by
@@ -386,11 +592,11 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
     __syncthreads();
     if (threadIdx.x == 0) {
       for (int i = 1; i < kSampleWarps; ++i) first = min(first, sh.warp_first[i]);
-      sh.pub.first = first;
+      sh.first = first;
     }
     cluster.sync();
     if (rank == 0 && threadIdx.x == 0) {
-      for (int r = 1; r < blocks; ++r) first = min(first, cluster.map_shared_rank(&sh.pub, r)->first);
+      for (int r = 1; r < blocks; ++r) first = min(first, *cluster.map_shared_rank(&sh.first, r));
       const bool none = best == -INFINITY;
       p.ids[row_id] = none ? -1 : first;
       if (p.logprobs) p.logprobs[row_id] = none ? -INFINITY : 0.0f;
@@ -414,92 +620,84 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
   kept.last = 0x7FFFFFFF;
 
   // ---- top-k ------------------------------------------------------------------------------
+  const int from = warp * row.chunk, to = min(row.n, from + row.chunk);
   if (top_k > 0 && top_k < p.vocab) {
-    __syncthreads();
-    clear_bins<false>(sh);
-    __syncthreads();
-    unsigned live = 0u;
+    unsigned beyond = 0u;  // in the last bin, where most tokens are: counted apart
     for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
       const float v = x[i];
       if (v == -INFINITY) continue;
-      ++live;
-      atomicAdd(&sh.count[row.bin(v)], 1u);
+      const int b = row.bin(v);
+      if (b == kBins - 1) ++beyond;
+      else atomicAdd(&sh.part[0][b], 1u);
     }
-    live = __reduce_add_sync(0xffffffffu, live);
-    if (lane == 0) sh.warp_sum[warp] = live;
-    if (cluster_total(sh, cluster) > (u64)top_k)
-      kept = select<false>(sh, cluster, row, weigh, kept, (u64)top_k);
-    else
-      cluster.sync();  // the counts above are read before the next sums replace them
+    beyond = __reduce_add_sync(0xffffffffu, beyond);
+    if (lane == 0 && beyond) atomicAdd(&sh.part[0][kBins - 1], beyond);
+    u64 live;
+    const Found found = find_bin<false>(sh, cluster, [&](u64) { return (u64)top_k; }, live);
+    if (found.bin >= 0 && live > (u64)top_k) {
+      if (found.before + found.amount <= (u64)kList) {
+        // all tokens up to the end of this bin: the first block of the cluster goes on alone
+        uint2* list = cluster.map_shared_rank(sh.list, 0);
+        unsigned* count = cluster.map_shared_rank(&sh.list_n[0], 0);
+        for (int i = from; i < to; i += 32) {
+          const float v = i + lane < to ? x[i + lane] : -INFINITY;
+          append(v != -INFINITY && row.bin(v) <= found.bin, descending_key(v), row.base + i + lane,
+                 list, count);
+        }
+        cluster.sync();
+        if (rank == 0) finish_list(sh, p, row_id, weigh, top_k, top_p, u);
+        return;
+      }
+      kept = select<false>(sh, cluster, row, weigh, kept, found.bin, (u64)top_k - found.before);
+    } else {
+      cluster.sync();  // the histogram has been read
+    }
+    clear_bins<true>(sh);
+    __syncthreads();
   }
 
   // ---- weights; top-p ---------------------------------------------------------------------
   const bool nucleus = top_p < 1.0f;
-  const int from = warp * row.chunk, to = min(row.n, from + row.chunk);
   u64 sum = 0ull;
-  if (nucleus) {
-    __syncthreads();
-    clear_bins<true>(sh);
-    __syncthreads();
-  }
   for (int i = from + lane; i < to; i += 32) {
     const float v = x[i];
     if (!kept.holds(descending_key(v), row.base + i)) continue;
     const u64 w = weigh(v);
-    if (w == 0ull) continue;
     sum += w;
-    if (nucleus) {
-      const int b = row.bin(v);
-      atomicAdd(&sh.mass[b], w);
-      atomicAdd(&sh.count[b], 1u);
-    }
+    if (nucleus && w) add_mass(sh, row.bin(v), w);
   }
-  __syncthreads();
-  sum = warp_total(sum);
-  if (lane == 0) sh.warp_sum[warp] = sum;
-  u64 total = cluster_total(sh, cluster);
+  u64 total = 0ull;
   if (nucleus) {
-    double need_d = ceil((double)fmaxf(top_p, 0.0f) * (double)total);
-    u64 need = need_d < 1.0 ? 1ull : (u64)need_d;
-    if (need < total) {
-      kept = select<true>(sh, cluster, row, weigh, kept, need);
+    const Found found =
+        find_bin<true>(sh, cluster, [&](u64 all) { return mass_needed(top_p, all); }, total);
+    const u64 need = mass_needed(top_p, total);
+    if (found.bin >= 0 && need < total) {
+      kept = select<true>(sh, cluster, row, weigh, kept, found.bin, need - found.before);
       sum = 0ull;
       for (int i = from + lane; i < to; i += 32) {
         const float v = x[i];
         if (kept.holds(descending_key(v), row.base + i)) sum += weigh(v);
       }
-      __syncthreads();
-      sum = warp_total(sum);
-      if (lane == 0) sh.warp_sum[warp] = sum;
-      total = cluster_total(sh, cluster);
     }
   }
+  sum = warp_total(sum);
+  if (lane == 0) sh.warp_sum[warp] = sum;
+  total = cluster_total(sh, cluster);
 
   // ---- draw -------------------------------------------------------------------------------
-  u64 target = u > 0.0f ? (u64)((double)fminf(u, 1.0f) * (double)total) : 0ull;
-  if (target >= total) target = total - 1ull;
+  const u64 target = draw_target(u, total);
   u64 before = 0ull;
-  for (int r = 0; r < rank; ++r) before += cluster.map_shared_rank(&sh.pub, r)->sum;
+  for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&sh.sum, r);
   for (int i = 0; i < warp; ++i) before += sh.warp_sum[i];
   if (before <= target && target < before + sum) {  // one warp of the cluster
     for (int i = from; i < to; i += 32) {
       const float v = i + lane < to ? x[i + lane] : -INFINITY;
       const u64 w = kept.holds(descending_key(v), row.base + i + lane) ? weigh(v) : 0ull;
-      u64 upto = w;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const u64 o = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += o;
-      }
+      const u64 upto = inclusive_scan(w);
       const unsigned past = __ballot_sync(0xffffffffu, before + upto > target);
       if (past) {
-        if (lane == __ffs(past) - 1) {
-          p.ids[row_id] = row.base + i + lane;
-          if (p.logprobs)
-            p.logprobs[row_id] =
-                (float)(weigh.exponent(v) * 0.69314718055994530942 -
-                        (log((double)total) - kWeightBits * 0.69314718055994530942));
-        }
+        if (lane == __ffs(past) - 1)
+          store_result(p, row_id, weigh, row.base + i + lane, v, total);
         break;
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
@@ -535,7 +733,7 @@ cudaError_t launch_sample(const void* logits, bool logits_f32, long long row_str
                                   (rows * blocks * 2 <= sm_count && vocab / blocks > 4096)))
     blocks *= 2;
   p.slice = (vocab + blocks - 1) / blocks;
-  const size_t bytes = sizeof(SampleShared) + (size_t)p.slice * sizeof(float);
+  const size_t bytes = sizeof(SampleShared) + (size_t)(p.slice + 3) * sizeof(float);
   const void* kernel = logits_f32 ? (const void*)sample_kernel<float>
                                   : (const void*)sample_kernel<__nv_bfloat16>;
   cudaError_t err =
