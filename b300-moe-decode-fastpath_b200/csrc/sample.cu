@@ -12,15 +12,14 @@
 // threshold on the logit and the index of the last token kept among those equal to it.  A
 // histogram over 2048 bins linear in m - x (for top-k of counts, for top-p of weights) finds the
 // bin in which the wanted sum is crossed; the few hundred tokens of that bin are collected in a
-// list and each is compared with all others of it.  Where top-k leaves few tokens altogether
-// they are collected instead, and one block does the rest.  A bin with more than 1024 tokens
+// list and sorted.  Where top-k leaves few tokens altogether they are collected instead, and one block does the rest.  A bin with more than 1024 tokens
 // (equal logits, a range far from that of the weights) is taken apart by three histograms over
 // the digits (11, 11 and 10 bits) of the logit's ordered bit pattern.  A row is read from memory
 // once and stays in the shared memory of a cluster of up to eight blocks, which exchange
 // histograms, lists and sums as distributed shared memory.
 //
 // What bounds it.  One to a few rows: the chain of load, four to five cluster barriers and two
-// passes over shared memory.  Many rows: the FP64 exponentials (14 instructions a token and
+// passes over shared memory.  Many rows: the FP64 exponentials (12 instructions a token and
 // pass) and the histogram's atomics.  Shared-memory atomics of 64 bits are loops of
 // compare-and-swap (9,000 to 16,000 cycles for 16,384 tokens, 240,000 where they meet in four
 // bins), those of 32 bits are not (1,300 and 4,300), so a weight is added as three parts of 15
@@ -30,9 +29,11 @@
 // sums resolve, and sums in another order would move them.  The weights are therefore integers,
 // w_i * 2^45 rounded to nearest: their sums are exact in 64 bits for up to 2^18 tokens, do not
 // depend on the order in which threads add them, and an atomic of integers leaves no trace of
-// who came first.  The exponential behind them is computed in FP64 to about 2^-52: reduction to
-// 2^(k/64) * 2^r with a table of 64 powers (Tang's table-driven scheme) and the Taylor
-// polynomial of degree 5 on |r| <= 2^-7.
+// who came first.  The exponential behind them is computed in FP64 to about 2^-49: reduction to
+// 2^(k/128) * 2^r with a table of 128 powers (Tang's table-driven scheme) and the Taylor
+// polynomial of degree 4 on |r| <= 2^-8.  A thread weighs four tokens at a time, without
+// branches: one after the other, each waiting for twelve dependent FP64 operations, they took
+// 15 us for 16,160 tokens of a block.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -48,7 +49,9 @@ constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kWeightBits = 45;
+constexpr int kPowers = 128;
 constexpr int kMaxCluster = 8;
+constexpr int kWide = 4;      // tokens that a thread weighs at a time
 constexpr uint32_t kMinusInfKey = 0xFF800000u;  // descending_key(-inf)
 
 struct SampleParams {
@@ -80,7 +83,8 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 // with at most 2^15 tokens in a block their sums stay within 32 bits.
 constexpr int kPartBits = 15;
 constexpr int kGroups = 64;            // groups of 32 bins
-constexpr int kList = 1024;            // tokens that are compared one by one
+constexpr int kList = 1024;            // tokens that are sorted
+constexpr int kPieces = 256;           // of a bin
 
 struct Found {
   int bin;      // -1: the whole histogram stays below what was asked for
@@ -93,7 +97,8 @@ struct alignas(16) SampleShared {
   uint2 list[kList];           // {key, index}; the cluster's in its first block
   u64 group[kGroups];          // of this block
   u64 group_total[kGroups];    // of the cluster
-  double power[64];
+  u64 bins[kMaxCluster][32];   // a group of bins of every block
+  double power[kPowers];
   u64 warp_sum[kSampleWarps];
   u64 sum;                     // what a block shows the others: sum, largest logit, an index
   float best;
@@ -102,49 +107,61 @@ struct alignas(16) SampleShared {
   Found found;
   float warp_best[kSampleWarps];
   int warp_first[kSampleWarps];
+  unsigned piece_n;
   uint32_t kept_key;
   int kept_last;
 };
 
-// FP32 -> FP64 by moving bits (zero and subnormal numbers come out within 2^-126, which is
-// nothing against the differences they enter); the conversion unit is four times slower
-__device__ __forceinline__ double widen(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const uint32_t hi = (u & 0x80000000u) | (((u & 0x7FFFFFFFu) >> 3) + 0x38000000u);
-  return __hiloint2double((int)hi, (int)(u << 29));
-}
-
 // exp of (x - best) / temperature as an integer multiple of 2^-45; `rate` is log2(e) / temperature
 struct Weigher {
-  const double* power;
+  const double* power;   // 2^(i/128 + 45)
   double best, rate;
   float best_f;
-  double least;  // min-p: smaller weights are dropped
+  float lowest;          // a logit whose weight rounds to zero (then also that of all below it)
+  bool bounded;          // there is such a logit, and the largest one is finite
+  double least;          // min-p: smaller weights are dropped
 
-  __device__ __forceinline__ double exponent(float x) const {
-    return x == best_f ? 0.0 : (widen(x) - best) * rate;
+  __device__ __forceinline__ void set(const double* power_, float best_, float temperature,
+                                      float min_p) {
+    power = power_;
+    best_f = best_;
+    best = (double)best_;
+    rate = 1.4426950408889634074 / (double)temperature;
+    lowest = best_ - 40.0f * temperature;  // 2^-57.7
+    bounded = isfinite(best_) && isfinite(lowest) && ((double)lowest - best) * rate < -48.0;
+    // min-p in units of 2^-45, not above the largest weight; NaN: off
+    least = min_p > 0.0f ? ldexp((double)fminf(min_p, 1.0f), kWeightBits) : 0.0;
   }
-  __device__ __forceinline__ u64 operator()(float x) const {
-    const double y = exponent(x);
-    if (!(y > -46.5)) return 0ull;  // rounds to zero; also -inf
-    // y = k / 64 + r: adding 1.5 * 2^46 leaves k in the low bits of the sum
-    const double magic = 105553116266496.0;
+  // y > -1000
+  __device__ __forceinline__ u64 power_of(double y) const {
+    // y = k / 128 + r: adding 1.5 * 2^45 leaves k in the low bits of the sum
+    const double magic = 52776558133248.0;
     const double shifted = y + magic;
     const int k = __double2loint(shifted);
-    const double z = (y - (shifted - magic)) * 0.69314718055994530942;
-    double e = fma(z, 1.0 / 120.0, 1.0 / 24.0);
-    e = fma(z, e, 1.0 / 6.0);
-    e = fma(z, e, 0.5);
-    e = fma(z, e, 1.0);
-    const double t = power[k & 63];
-    const double v = fma(t * z, e, t);          // 2^(k mod 64 / 64 + r)
-    // times 2^(floor(k / 64) + 45) through the exponent field
-    const double w =
-        __hiloint2double(__double2hiint(v) + ((k >> 6) + kWeightBits) * (1 << 20), __double2loint(v));
-    if (w < least) return 0ull;
+    const double r = y - (shifted - magic);
+    // 2^r = 1 + r (c1 + r (c2 + r (c3 + r c4))), cn = ln(2)^n / n!
+    constexpr double c1 = 0.69314718055994530942;
+    constexpr double c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
+    double e = fma(r, c4, c3);
+    e = fma(r, e, c2);
+    e = fma(r, e, c1);
+    const double t = power[k & (kPowers - 1)];
+    const double v = fma(t * r, e, t);          // 2^(k mod 128 / 128 + r + 45)
+    // times 2^floor(k / 128) through the exponent field
+    const double w = __hiloint2double(
+        __double2hiint(v) + (int)(((unsigned)k & ~(unsigned)(kPowers - 1)) << 13), __double2loint(v));
     // round to an integer in the low bits: w <= 2^45
-    const double rounded = w + 4503599627370496.0;
-    return (u64)__double_as_longlong(rounded) & ((1ull << 52) - 1ull);
+    const u64 n = (u64)__double_as_longlong(w + 4503599627370496.0) & ((1ull << 52) - 1ull);
+    return least > 0.0 && w < least ? 0ull : n;
+  }
+  __device__ __forceinline__ double exponent(float x) const {
+    return x == best_f ? 0.0 : ((double)x - best) * rate;
+  }
+  // any logit but NaN; -inf: 0
+  __device__ __forceinline__ u64 operator()(float x) const {
+    if (bounded) return power_of(((double)fmaxf(x, lowest) - best) * rate);
+    const double y = exponent(x);
+    return x != -INFINITY && y > -48.0 ? power_of(y) : 0ull;
   }
 };
 
@@ -164,6 +181,20 @@ struct Row {
   float best, scale;   // linear bins: (best - x) * scale
   __device__ __forceinline__ int bin(float v) const {
     return v == best ? 0 : min(kBins - 1, (int)((best - v) * scale));
+  }
+  // whether bin(v) == b, for a bin's borders as numbers
+  __device__ __forceinline__ bool in_bin(float v, int b) const {
+    const float t = v == best ? 0.0f : (best - v) * scale;
+    return t >= (float)b && (t < (float)(b + 1) || b == kBins - 1);
+  }
+  // and up to bin b
+  __device__ __forceinline__ bool upto_bin(float v, int b) const {
+    return v == best || (best - v) * scale < (float)(b + 1) || b == kBins - 1;
+  }
+  // the part of bin b that v lies in, of kPieces
+  __device__ __forceinline__ int piece(float v, int b) const {
+    const float t = v == best ? 0.0f : (best - v) * scale;
+    return max(0, min(kPieces - 1, (int)((t - (float)b) * (float)kPieces)));
   }
 };
 
@@ -187,7 +218,9 @@ __device__ __forceinline__ u64 cluster_total(SampleShared& sh, cg::cluster_group
   if (threadIdx.x == 0) sh.sum = mine;
   cluster.sync();
   u64 s = 0ull;
-  for (unsigned r = 0; r < cluster.num_blocks(); ++r) s += *cluster.map_shared_rank(&sh.sum, r);
+#pragma unroll
+  for (unsigned r = 0; r < kMaxCluster; ++r)
+    if (r < cluster.num_blocks()) s += *cluster.map_shared_rank(&sh.sum, r);
   return s;
 }
 
@@ -228,11 +261,14 @@ __device__ Found find_bin(SampleShared& sh, cg::cluster_group& cluster, Need nee
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int blocks = (int)cluster.num_blocks();
   __syncthreads();
+  {  // four bins per thread, eight threads per group
+    static_assert(kBins == 4 * kSampleThreads && kBins == 32 * kGroups, "bins per thread");
+    u64 v = 0ull;
 #pragma unroll
-  for (int i = 0; i < kGroups / kSampleWarps; ++i) {
-    const int group = warp * (kGroups / kSampleWarps) + i;
-    const u64 v = warp_total(bin_amount<BY_MASS>(sh.part, group * 32 + lane));
-    if (lane == 0) sh.group[group] = v;
+    for (int i = 0; i < 4; ++i) v += bin_amount<BY_MASS>(sh.part, 4 * threadIdx.x + i);
+#pragma unroll
+    for (int m = 4; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    if ((threadIdx.x & 7) == 0) sh.group[threadIdx.x / 8] = v;
   }
   cluster.sync();
   {  // as many neighbouring lanes as there are blocks share a group
@@ -259,11 +295,13 @@ __device__ Found find_bin(SampleShared& sh, cg::cluster_group& cluster, Need nee
     before += first;
     ++group;
   }
+  const int bin = group * 32 + lane;
+  if (warp < blocks)  // one warp per block of the cluster: a single trip
+    sh.bins[warp][lane] = bin_amount<BY_MASS>(cluster.map_shared_rank(sh.part, warp), bin);
+  __syncthreads();
   if (warp == 0) {
-    const int bin = group * 32 + lane;
     u64 v = 0ull;
-    for (int r = 0; r < blocks; ++r)
-      v += bin_amount<BY_MASS>(cluster.map_shared_rank(sh.part, r), bin);
+    for (int r = 0; r < blocks; ++r) v += sh.bins[r][lane];
     const u64 run = before + inclusive_scan(v);
     if (lane == __ffs(__ballot_sync(0xffffffffu, run >= need)) - 1) {
       sh.found.bin = bin;
@@ -288,6 +326,65 @@ __device__ __forceinline__ void append(bool chosen, uint32_t key, int index, uin
   const unsigned at = base + __popc(votes & ((1u << lane) - 1u));
   if (chosen && at < (unsigned)kList) list[at] = make_uint2(key, (unsigned)index);
 }
+// Sorts `count` integers, two per thread (2 t and 2 t + 1), ascending; what is behind them must be
+// ~0.  A bitonic network: partners within a warp exchange by shuffles, others through `scratch`
+// (two integers per thread).  Threads without a share only keep the barriers.
+__device__ __forceinline__ void sort_block(u64 (&v)[2], int count, ulonglong2* scratch) {
+  const int t = threadIdx.x;
+  const int padded = max(2, count <= 1 ? 1 : 1 << (32 - __clz(count - 1)));
+  const bool in = 2 * (t & ~31) < padded;  // whole warps
+  for (int size = 2; size <= padded; size <<= 1) {
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      const bool up = (2 * t & size) == 0;
+      if (stride >= 64) {
+        __syncthreads();
+        if (in) scratch[t] = make_ulonglong2(v[0], v[1]);
+        __syncthreads();
+      }
+      if (!in) continue;
+      if (stride == 1) {
+        const bool ascending = size == 2 ? (t & 1) == 0 : up;
+        if ((v[0] > v[1]) == ascending) {
+          const u64 x = v[0];
+          v[0] = v[1];
+          v[1] = x;
+        }
+        continue;
+      }
+      const bool low = (2 * t & stride) == 0;  // keeps the smaller of the two where ascending
+      u64 other[2];
+      if (stride >= 64) {
+        const ulonglong2 o = scratch[t ^ (stride >> 1)];
+        other[0] = o.x;
+        other[1] = o.y;
+      } else {
+        other[0] = __shfl_xor_sync(0xffffffffu, v[0], stride >> 1);
+        other[1] = __shfl_xor_sync(0xffffffffu, v[1], stride >> 1);
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        if ((other[q] < v[q]) == (low == up)) v[q] = other[q];
+    }
+  }
+}
+// Sum of v over the threads before this one, and over all.
+__device__ __forceinline__ u64 block_scan(SampleShared& sh, u64 v, u64& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 upto = inclusive_scan(v);
+  __syncthreads();  // the sums before have been read
+  if (lane == 31) sh.warp_sum[warp] = upto;
+  __syncthreads();
+  u64 before = 0ull;
+  total = 0ull;
+#pragma unroll
+  for (int i = 0; i < kSampleWarps; ++i) {
+    const u64 w = sh.warp_sum[i];
+    if (i < warp) before += w;
+    total += w;
+  }
+  return before + upto - v;
+}
+// (logit, index) as one integer, in the order of the tokens
 __device__ __forceinline__ u64 place(const uint2& e) { return ((u64)e.x << 32) | e.y; }
 
 // The shortest prefix of the kept tokens whose sum (of counts, or of weights) ends in bin
@@ -300,35 +397,88 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
   // the bin's tokens
   uint2* list = cluster.map_shared_rank(sh.list, 0);
   unsigned* count = cluster.map_shared_rank(&sh.list_n[BY_MASS], 0);
-  for (int i = from; i < to; i += 32) {
-    const float v = i + lane < to ? row.x[i + lane] : -INFINITY;
-    const uint32_t key = descending_key(v);
-    append(v != -INFINITY && row.bin(v) == bin && kept.holds(key, row.base + i + lane), key,
-           row.base + i + lane, list, count);
+  for (int i = from + lane; i - lane < to; i += 32 * kWide) {
+    float v[kWide];
+    bool chosen[kWide], any = false;
+#pragma unroll
+    for (int j = 0; j < kWide; ++j) {
+      v[j] = i + 32 * j < to ? row.x[i + 32 * j] : -INFINITY;
+      chosen[j] = v[j] != -INFINITY && row.in_bin(v[j], bin);
+      any |= chosen[j];
+    }
+    if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+    for (int j = 0; j < kWide; ++j) {
+      const uint32_t key = descending_key(v[j]);
+      const int index = row.base + i + 32 * j;
+      append(chosen[j] && kept.holds(key, index), key, index, list, count);
+    }
   }
   cluster.sync();
   const unsigned n = *count;
   Kept next;
   if (n <= (unsigned)kList) {
-    // a copy of the list, with the weights behind it, where the histogram was
-    uint2* own = reinterpret_cast<uint2*>(&sh.part[0][0]);
-    u64* weight = reinterpret_cast<u64*>(&sh.part[1][0]);
-    static_assert(kList * sizeof(uint2) == sizeof(sh.part[0]) &&
-                      kList * sizeof(u64) == sizeof(sh.part[0]), "they fit");
-    for (unsigned i = threadIdx.x; i < n; i += kSampleThreads) {
-      own[i] = list[i];
-      weight[i] = BY_MASS ? weigh(logit_of(own[i].x)) : 1ull;
+    // A histogram of the list over 256 pieces of the bin narrows it down to the tokens of one
+    // piece, mostly one or two; those are sorted.  Every block does this for itself.
+    static_assert(kList <= 2 * kSampleThreads, "two tokens per thread");
+    if (threadIdx.x < kPieces) sh.part[0][threadIdx.x] = sh.part[1][threadIdx.x] = sh.part[2][threadIdx.x] = 0u;
+    if (threadIdx.x == 0) sh.piece_n = 0u;
+    __syncthreads();
+    uint2 e[2];
+    u64 w[2];
+    int piece[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const unsigned i = threadIdx.x + q * kSampleThreads;
+      w[q] = 0ull;
+      piece[q] = -1;
+      if (i >= n) continue;
+      e[q] = list[i];
+      const float v = logit_of(e[q].x);
+      w[q] = BY_MASS ? weigh(v) : 1ull;
+      piece[q] = row.piece(v, bin);
+      if (w[q]) add_mass(sh, piece[q], w[q]);
     }
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < n; i += kSampleThreads) {
-      const u64 mine = place(own[i]);
-      u64 before = 0ull;
-#pragma unroll 4
-      for (unsigned j = 0; j < n; ++j) before += place(own[j]) < mine ? weight[j] : 0ull;
-      if (before < rest && before + weight[i] >= rest) {
-        sh.kept_key = own[i].x;
-        sh.kept_last = (int)own[i].y;
+    // every warp: eight pieces per lane
+    u64 amount[kPieces / 32], sum = 0ull;
+#pragma unroll
+    for (int i = 0; i < kPieces / 32; ++i) {
+      amount[i] = bin_amount<true>(sh.part, lane * (kPieces / 32) + i);
+      sum += amount[i];
+    }
+    u64 run = inclusive_scan(sum) - sum;
+    int mine = -1;
+    if (run < rest && run + sum >= rest) {
+#pragma unroll
+      for (int i = 0; i < kPieces / 32; ++i) {
+        if (mine >= 0) break;
+        if (run + amount[i] >= rest) mine = lane * (kPieces / 32) + i;
+        else run += amount[i];
       }
+    }
+    const int at = __ffs(__ballot_sync(0xffffffffu, mine >= 0)) - 1;
+    mine = __shfl_sync(0xffffffffu, mine, at);
+    rest -= __shfl_sync(0xffffffffu, run, at);
+    u64* some = reinterpret_cast<u64*>(&sh.part[1][0]);  // behind the pieces of part[0], and in
+    __syncthreads();                                     // place of the others
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (piece[q] == mine) some[atomicAdd(&sh.piece_n, 1u)] = place(e[q]);
+    __syncthreads();
+    const int m = (int)sh.piece_n;
+    u64 v[2], total;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) v[q] = 2 * threadIdx.x + q < m ? some[2 * threadIdx.x + q] : ~0ull;
+    sort_block(v, m, reinterpret_cast<ulonglong2*>(&sh.part[1][0]));
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      w[q] = v[q] == ~0ull ? 0ull : BY_MASS ? weigh(logit_of((uint32_t)(v[q] >> 32))) : 1ull;
+    const u64 before = block_scan(sh, w[0] + w[1], total);
+    if (before < rest && before + w[0] + w[1] >= rest) {
+      const u64 last = before + w[0] >= rest ? v[0] : v[1];
+      sh.kept_key = (uint32_t)(last >> 32);
+      sh.kept_last = (int)(uint32_t)last;
     }
     __syncthreads();
     next.key = sh.kept_key;
@@ -424,65 +574,48 @@ __device__ __forceinline__ void store_result(const SampleParams& p, int row_id,
                                  (log((double)total) - kWeightBits * 0.69314718055994530942));
 }
 
-// All that is left after top-k fits the list: one block cuts it to k tokens, weighs them, cuts to
-// top-p and draws, comparing every token with every other.
+// All that is left after top-k fits the list: one block sorts it, cuts it to k tokens, weighs them,
+// cuts to top-p, and sorts what is left by index for the draw.
 __device__ void finish_list(SampleShared& sh, const SampleParams& p, int row_id,
                             const Weigher& weigh, int top_k, float top_p, float u) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = (int)sh.list_n[0];
-  constexpr int kEach = kList / kSampleThreads;
-  u64* weight = reinterpret_cast<u64*>(&sh.part[0][0]);
-  for (int i = threadIdx.x; i < n; i += kSampleThreads) weight[i] = weigh(logit_of(sh.list[i].x));
-  __syncthreads();
-  u64 mine[kEach], before[kEach], sum = 0ull;
+  const int n = (int)sh.list_n[0], at = 2 * threadIdx.x;
+  ulonglong2* scratch = reinterpret_cast<ulonglong2*>(&sh.part[0][0]);
+  u64* entry = reinterpret_cast<u64*>(&sh.part[2][0]);
+  u64 v[2], w[2], total;
 #pragma unroll
-  for (int q = 0; q < kEach; ++q) {
-    const int i = threadIdx.x + q * kSampleThreads;
-    mine[q] = before[q] = 0ull;
-    if (i >= n) continue;
-    const u64 at = place(sh.list[i]);
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j)
-      if (place(sh.list[j]) < at) {
-        ++rank;
-        before[q] += weight[j];
-      }
-    if (rank < top_k) mine[q] = weight[i];
-    sum += mine[q];
-  }
-  sum = warp_total(sum);
-  if (lane == 0) sh.warp_sum[warp] = sum;
-  u64 total = block_total(sh);  // and all weights have been read
+  for (int q = 0; q < 2; ++q) v[q] = at + q < n ? place(sh.list[at + q]) : ~0ull;
+  sort_block(v, n, scratch);
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+    w[q] = at + q < n && at + q < top_k ? weigh(logit_of((uint32_t)(v[q] >> 32))) : 0ull;
+  u64 before = block_scan(sh, w[0] + w[1], total);
   if (top_p < 1.0f) {
     const u64 need = mass_needed(top_p, total);
-    __syncthreads();
-    sum = 0ull;
-#pragma unroll
-    for (int q = 0; q < kEach; ++q) {
-      if (before[q] >= need) mine[q] = 0ull;
-      sum += mine[q];
-    }
-    sum = warp_total(sum);
-    if (lane == 0) sh.warp_sum[warp] = sum;
-    total = block_total(sh);
+    if (before + w[0] >= need) w[1] = 0ull;
+    if (before >= need) w[0] = 0ull;
   }
+  // {index, place in the order}; what is not kept goes to the end
 #pragma unroll
-  for (int q = 0; q < kEach; ++q) {
-    const int i = threadIdx.x + q * kSampleThreads;
-    if (i < n) weight[i] = mine[q];
+  for (int q = 0; q < 2; ++q) {
+    entry[at + q] = v[q];
+    v[q] = w[q] ? (v[q] << 32) | (unsigned)(at + q) : ~0ull;
   }
   __syncthreads();
-  const u64 target = draw_target(u, total);
+  sort_block(v, n, scratch);
+  float x[2];
+  int index[2];
 #pragma unroll
-  for (int q = 0; q < kEach; ++q) {
-    if (mine[q] == 0ull) continue;
-    const uint2 e = sh.list[threadIdx.x + q * kSampleThreads];
-    u64 run = 0ull;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) run += sh.list[j].y < e.y ? weight[j] : 0ull;
-    if (run <= target && target < run + mine[q])
-      store_result(p, row_id, weigh, (int)e.y, logit_of(e.x), total);
+  for (int q = 0; q < 2; ++q) {
+    const u64 e = v[q] != ~0ull ? entry[(unsigned)v[q]] : 0ull;
+    x[q] = logit_of((uint32_t)(e >> 32));
+    index[q] = (int)(uint32_t)e;
+    w[q] = v[q] != ~0ull ? weigh(x[q]) : 0ull;
+  }
+  before = block_scan(sh, w[0] + w[1], total);
+  const u64 target = draw_target(u, total);
+  if (before <= target && target < before + w[0] + w[1]) {
+    const int q = target < before + w[0] ? 0 : 1;
+    store_result(p, row_id, weigh, index[q], x[q], total);
   }
 }
 
@@ -564,7 +697,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   float* x = reinterpret_cast<float*>(smem + sizeof(SampleShared)) + ((4 - head_of(src)) & 3);
   row.x = x;
   clear_bins<true>(sh);
-  if (threadIdx.x < 64) sh.power[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+  if (threadIdx.x < kPowers) sh.power[threadIdx.x] = exp2((double)threadIdx.x / kPowers + kWeightBits);
   if (threadIdx.x < 2) sh.list_n[threadIdx.x] = 0u;
   float best = load_row<T>(src, row.n, x);
 #pragma unroll
@@ -577,7 +710,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   }
   cluster.sync();
   best = -INFINITY;
-  for (int r = 0; r < blocks; ++r) best = fmaxf(best, *cluster.map_shared_rank(&sh.best, r));
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; ++r)
+    if (r < blocks) best = fmaxf(best, *cluster.map_shared_rank(&sh.best, r));
   row.best = best;
 
   if (best == -INFINITY || !(temperature > 0.0f)) {  // nothing to draw, or nothing to draw by
@@ -606,18 +741,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   }
 
   Weigher weigh;
-  weigh.power = sh.power;
-  weigh.best = widen(best);
-  weigh.best_f = best;
-  weigh.rate = 1.4426950408889634074 / (double)temperature;
-  // min-p in units of 2^-45; not above the largest weight, NaN: off
-  weigh.least = min_p > 0.0f ? ldexp((double)fminf(min_p, 1.0f), kWeightBits) : 0.0;
+  weigh.set(sh.power, best, temperature, min_p);
   // 2047 linear bins over the range of logits whose weight is not zero, one for the rest
   row.scale = fminf((float)(2047.0 / 32.3) / temperature, 3.0e38f);
 
   Kept kept;
   kept.key = kMinusInfKey - 1u;  // every logit above -inf
   kept.last = 0x7FFFFFFF;
+  bool all = true;               // as long as that is so, the weights alone tell
 
   // ---- top-k ------------------------------------------------------------------------------
   const int from = warp * row.chunk, to = min(row.n, from + row.chunk);
@@ -639,16 +770,26 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
         // all tokens up to the end of this bin: the first block of the cluster goes on alone
         uint2* list = cluster.map_shared_rank(sh.list, 0);
         unsigned* count = cluster.map_shared_rank(&sh.list_n[0], 0);
-        for (int i = from; i < to; i += 32) {
-          const float v = i + lane < to ? x[i + lane] : -INFINITY;
-          append(v != -INFINITY && row.bin(v) <= found.bin, descending_key(v), row.base + i + lane,
-                 list, count);
+        for (int i = from + lane; i - lane < to; i += 32 * kWide) {
+          float v[kWide];
+          bool chosen[kWide], any = false;
+#pragma unroll
+          for (int j = 0; j < kWide; ++j) {
+            v[j] = i + 32 * j < to ? x[i + 32 * j] : -INFINITY;
+            chosen[j] = v[j] != -INFINITY && row.upto_bin(v[j], found.bin);
+            any |= chosen[j];
+          }
+          if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+          for (int j = 0; j < kWide; ++j)
+            append(chosen[j], descending_key(v[j]), row.base + i + 32 * j, list, count);
         }
         cluster.sync();
         if (rank == 0) finish_list(sh, p, row_id, weigh, top_k, top_p, u);
         return;
       }
       kept = select<false>(sh, cluster, row, weigh, kept, found.bin, (u64)top_k - found.before);
+      all = false;
     } else {
       cluster.sync();  // the histogram has been read
     }
@@ -659,12 +800,26 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   // ---- weights; top-p ---------------------------------------------------------------------
   const bool nucleus = top_p < 1.0f;
   u64 sum = 0ull;
-  for (int i = from + lane; i < to; i += 32) {
-    const float v = x[i];
-    if (!kept.holds(descending_key(v), row.base + i)) continue;
-    const u64 w = weigh(v);
-    sum += w;
-    if (nucleus && w) add_mass(sh, row.bin(v), w);
+  for (int i = from + lane; i < to; i += 32 * kWide) {
+    float v[kWide];
+    u64 w[kWide];
+#pragma unroll
+    for (int j = 0; j < kWide; ++j) {
+      v[j] = i + 32 * j < to ? x[i + 32 * j] : -INFINITY;
+      w[j] = weigh(v[j]);
+    }
+    if (!all) {
+#pragma unroll
+      for (int j = 0; j < kWide; ++j)
+        if (!kept.holds(descending_key(v[j]), row.base + i + 32 * j)) w[j] = 0ull;
+    }
+#pragma unroll
+    for (int j = 0; j < kWide; ++j) sum += w[j];
+    if (nucleus) {
+#pragma unroll
+      for (int j = 0; j < kWide; ++j)
+        if (w[j]) add_mass(sh, row.bin(v[j]), w[j]);
+    }
   }
   u64 total = 0ull;
   if (nucleus) {
@@ -673,10 +828,23 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     const u64 need = mass_needed(top_p, total);
     if (found.bin >= 0 && need < total) {
       kept = select<true>(sh, cluster, row, weigh, kept, found.bin, need - found.before);
+      all = false;
       sum = 0ull;
-      for (int i = from + lane; i < to; i += 32) {
-        const float v = x[i];
-        if (kept.holds(descending_key(v), row.base + i)) sum += weigh(v);
+      for (int i = from + lane; i < to; i += 32 * kWide) {
+        bool wanted[kWide], any = false;
+        float v[kWide];
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) {
+          v[j] = i + 32 * j < to ? x[i + 32 * j] : -INFINITY;
+          wanted[j] = kept.holds(descending_key(v[j]), row.base + i + 32 * j);
+          any |= wanted[j];
+        }
+        if (!any) continue;
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) {
+          const u64 w = weigh(v[j]);
+          sum += wanted[j] ? w : 0ull;
+        }
       }
     }
   }
@@ -688,22 +856,32 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   const u64 target = draw_target(u, total);
   u64 before = 0ull;
   for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&sh.sum, r);
-  for (int i = 0; i < warp; ++i) before += sh.warp_sum[i];
-  if (before <= target && target < before + sum) {  // one warp of the cluster
-    for (int i = from; i < to; i += 32) {
-      const float v = i + lane < to ? x[i + lane] : -INFINITY;
-      const u64 w = kept.holds(descending_key(v), row.base + i + lane) ? weigh(v) : 0ull;
-      const u64 upto = inclusive_scan(w);
-      const unsigned past = __ballot_sync(0xffffffffu, before + upto > target);
-      if (past) {
-        if (lane == __ffs(past) - 1)
-          store_result(p, row_id, weigh, row.base + i + lane, v, total);
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
+  cluster.sync();  // no block leaves while another reads its shared memory
+  if (before <= target && target < before + sh.sum) {  // one block of the cluster
+    // the warp whose tokens hold the target; its tokens, one per thread
+    int owner = 0;
+    for (; owner < kSampleWarps - 1; ++owner) {
+      const u64 w = sh.warp_sum[owner];
+      if (target < before + w) break;
+      before += w;
+    }
+    const int first = owner * row.chunk, end = min(row.n, first + row.chunk);
+    for (int start = first; start < end; start += kSampleThreads) {
+      const int i = start + threadIdx.x;
+      const float v = i < end ? x[i] : -INFINITY;
+      u64 w = weigh(v);
+      if (!all && !kept.holds(descending_key(v), row.base + i)) w = 0ull;
+      u64 upto = inclusive_scan(w);
+      __syncthreads();  // the sums before have been read
+      if (lane == 31) sh.warp_sum[warp] = upto;
+      __syncthreads();
+      upto += before;
+      for (int k = 0; k < warp; ++k) upto += sh.warp_sum[k];
+      if (w && upto - w <= target && target < upto)
+        store_result(p, row_id, weigh, row.base + i, v, total);
+      for (int k = 0; k < kSampleWarps; ++k) before += sh.warp_sum[k];
     }
   }
-  cluster.sync();  // no block leaves while another reads its shared memory
 }
 
 }  // namespace
