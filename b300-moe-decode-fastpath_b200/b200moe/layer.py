@@ -10,6 +10,8 @@ reference.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -63,14 +65,20 @@ def _validate(hidden_states, router_weight, gate_up, down, scales, num_experts: 
         raise TypeError("router_weight must have dtype torch.bfloat16 or torch.float32")
     if gate_up.dtype != kind or down.dtype != kind:
         raise TypeError(f"gate_up_weight and down_weight must have dtype {kind}")
-    if scales is not None and any(s.dtype != torch.float32 for s in scales):
+    if scales is not None and (scales[0].dtype is not torch.float32
+                               or scales[1].dtype is not torch.float32):
         raise TypeError("scales must have dtype torch.float32")
-    tensors = (hidden_states, router_weight, gate_up, down) + (scales or ())
-    if any(t.device != hidden_states.device for t in tensors):
+    device = hidden_states.device
+    if router_weight.device != device or gate_up.device != device or down.device != device or \
+            (scales is not None and (scales[0].device != device or scales[1].device != device)):
         raise ValueError("all inputs must be on the same device")
-    if not all(t.is_contiguous() for t in tensors):
+    if not (hidden_states.is_contiguous() and router_weight.is_contiguous()
+            and gate_up.is_contiguous() and down.is_contiguous()
+            and (scales is None or scales[0].is_contiguous() and scales[1].is_contiguous())):
         raise ValueError("all inputs must be contiguous")
-    if any(t.requires_grad for t in tensors):
+    if hidden_states.requires_grad or router_weight.requires_grad or gate_up.requires_grad or \
+            down.requires_grad or \
+            (scales is not None and (scales[0].requires_grad or scales[1].requires_grad)):
         raise ValueError("the one-kernel layer does not support autograd")
     if hidden % step or inter % step:
         raise ValueError(f"hidden_size and intermediate_size must be divisible by {step}")
@@ -80,19 +88,34 @@ def _validate(hidden_states, router_weight, gate_up, down, scales, num_experts: 
     return RoutedMoEShape(tokens, num_experts, top_k, hidden, inter)
 
 
-def _enqueue_layer(args, router_weight, ids, weights, device: torch.device) -> None:
-    fn = _lib.load().b200moe_layer
-    call = (args, router_weight.data_ptr(), router_weight.dtype is torch.float32,
-            None if ids is None else ids.data_ptr(),
-            None if weights is None else weights.data_ptr(),
-            torch._C._cuda_getCurrentRawStream(device.index))
-    if torch.cuda.current_device() == device.index:
-        code = fn(*call)
-    else:
-        with torch.cuda.device(device):
-            code = fn(*call)
-    if code:
-        _lib.check(code, "b200moe_layer")
+class _Binding:
+    """What a workspace keeps for this entry point from one :meth:`reserve` to the next: the
+    argument struct with the dimensions and scratch filled in, and the stream of the last use."""
+
+    __slots__ = ("key", "allocations", "tokens", "stream", "stream_ptr", "args", "ref")
+
+
+def _bind(workspace: B300MoEWorkspace, key, hidden_states, gate_up, down,
+          shape: RoutedMoEShape) -> _Binding:
+    """Reserves the workspace for this call, by its own rules, and binds an argument struct."""
+
+    device = hidden_states.device
+    workspace.reserve(
+        num_tokens=shape.num_tokens, num_experts=shape.num_experts, top_k=shape.top_k,
+        hidden_size=shape.hidden_size, intermediate_size=shape.intermediate_size,
+        device=device, dtype=torch.bfloat16, backend="b200_bf16", quant_mode="bf16")
+    b = _Binding()
+    b.key, b.allocations, b.tokens = key, workspace.allocation_count, workspace._tokens
+    b.stream = torch.cuda.current_stream(device)
+    b.stream_ptr = int(b.stream.cuda_stream)
+    # a copy: the struct that the workspace caches is bound to the last call's weights.  The
+    # routing tensors of the struct are not read by this entry point.
+    b.args = _lib.B200MoeArgs.from_buffer_copy(
+        _native_args(hidden_states, hidden_states, hidden_states, gate_up, down, shape, workspace,
+                     None, 0))
+    b.ref = ctypes.byref(b.args)
+    workspace._layer_binding = b
+    return b
 
 
 def _run(hidden_states, router_weight, gate_up, down, scales, shape: RoutedMoEShape,
@@ -100,27 +123,57 @@ def _run(hidden_states, router_weight, gate_up, down, scales, shape: RoutedMoESh
          out: torch.Tensor | None):
     if workspace is not None and not isinstance(workspace, B300MoEWorkspace):
         raise TypeError("workspace must be a B300MoEWorkspace or None")
-    _resolve_native_backend("b200_bf16" if scales is None else "b200_fp8", hidden_states,
-                            router_weight, gate_up, down, shape)
     device = hidden_states.device
     active = workspace if workspace is not None else B300MoEWorkspace(device=device)
+    key = (device, shape.num_experts, shape.top_k, shape.hidden_size, shape.intermediate_size)
+    tokens = shape.num_tokens
     with active._lock:
-        active.reserve(
-            num_tokens=shape.num_tokens, num_experts=shape.num_experts, top_k=shape.top_k,
-            hidden_size=shape.hidden_size, intermediate_size=shape.intermediate_size,
-            device=device, dtype=torch.bfloat16, backend="b200_bf16", quant_mode="bf16")
+        b = active._layer_binding
+        # the same layout and stream as the last time, and no capture: nothing to reserve
+        repeated = (b is not None and b.key == key and b.allocations == active._allocations
+                    and tokens <= b.tokens and active._last_stream == b.stream_ptr
+                    and torch._C._cuda_getCurrentRawStream(device.index) == b.stream_ptr
+                    and not torch._C._cuda_isCurrentStreamCapturing())
+        if repeated:
+            active._reuses += 1
+            active._last_reused = True
+            active._last_shape = (tokens, shape.num_experts, shape.top_k, shape.hidden_size,
+                                  shape.intermediate_size)
+        else:
+            _resolve_native_backend("b200_bf16" if scales is None else "b200_fp8", hidden_states,
+                                    router_weight, gate_up, down, shape)
+            b = _bind(active, key, hidden_states, gate_up, down, shape)
         output = out if out is not None else torch.empty_like(hidden_states)
         ids = weights = None
         if return_routing:
-            ids = torch.empty(shape.num_tokens, shape.top_k, dtype=torch.int64, device=device)
-            weights = torch.empty(shape.num_tokens, shape.top_k, device=device)
-        # the routing tensors of the struct are not read by this entry point
-        args = _native_args(hidden_states, hidden_states, hidden_states, gate_up, down, shape,
-                            active, output, 0 if scales is None else _lib.FLAG_FP8_WEIGHTS)
-        if scales is not None:
+            ids = torch.empty(tokens, shape.top_k, dtype=torch.int64, device=device)
+            weights = torch.empty(tokens, shape.top_k, device=device)
+        args = b.args
+        args.hidden_states = hidden_states.data_ptr()
+        args.gate_up_weight, args.down_weight = gate_up.data_ptr(), down.data_ptr()
+        args.num_tokens = tokens
+        args.output = output.data_ptr()
+        if scales is None:
+            args.flags = 0
+        else:
+            args.flags = _lib.FLAG_FP8_WEIGHTS
             args.gate_up_scale, args.down_scale = scales[0].data_ptr(), scales[1].data_ptr()
-        _enqueue_layer(args, router_weight, ids, weights, device)
-        active._record_use()
+        call = (b.ref, router_weight.data_ptr(), router_weight.dtype is torch.float32,
+                None if ids is None else ids.data_ptr(),
+                None if weights is None else weights.data_ptr(),
+                torch._C._cuda_getCurrentRawStream(device.index))
+        fn = _lib.load().b200moe_layer
+        if torch._C._cuda_getDevice() == device.index:
+            code = fn(*call)
+        else:
+            with torch.cuda.device(device):
+                code = fn(*call)
+        if code:
+            _lib.check(code, "b200moe_layer")
+        if repeated:
+            active._event.record(b.stream)
+        else:
+            active._record_use()
         if check_status:
             active.raise_for_status()
     return (output, ids, weights) if return_routing else output

@@ -23,97 +23,107 @@ def _check_buffer(name: str, t: object, shape, dtype: torch.dtype, device: torch
 
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor or None")
-    if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous() \
+    if t.shape != shape or t.dtype is not dtype or t.device != device or not t.is_contiguous() \
             or t.requires_grad:
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on "
                          f"{device} that does not require grad")
 
 
-def _check(hidden_states, residual, weight, eps, step: int) -> None:
-    for name, t in (("hidden_states", hidden_states), ("weight", weight)):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
+def _check(x, residual, weight, eps, step: int) -> int:
+    """Checks of the inputs; the number of rows.  Written out flat: a decode step calls this once
+    per layer, and its host time is of the order of the kernel's."""
+
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("hidden_states must be a torch.Tensor")
+    if not isinstance(weight, torch.Tensor):
+        raise TypeError("weight must be a torch.Tensor")
     if residual is not None and not isinstance(residual, torch.Tensor):
         raise TypeError("residual must be a torch.Tensor or None")
-    if isinstance(eps, bool) or not isinstance(eps, (int, float)):
+    if type(eps) is not float and (isinstance(eps, bool) or not isinstance(eps, (int, float))):
         raise TypeError("eps must be a number")
-    if not (eps >= 0.0 and math.isfinite(eps)):
+    if not 0.0 <= eps < math.inf:
         raise ValueError("eps must be finite and not negative")
-    if hidden_states.ndim < 1:
+    shape = x.shape
+    if len(shape) < 1:
         raise ValueError("hidden_states must have shape [..., hidden_size]")
-    hidden = hidden_states.shape[-1]
+    hidden = shape[-1]
     if weight.shape != (hidden,):
         raise ValueError("weight must have shape [hidden_size]")
-    if residual is not None and residual.shape != hidden_states.shape:
+    if residual is not None and residual.shape != shape:
         raise ValueError("residual and hidden_states must have the same shape")
-    if hidden_states.dtype is not torch.bfloat16:
+    if x.dtype is not torch.bfloat16:
         raise TypeError("hidden_states must have dtype torch.bfloat16")
     if weight.dtype not in _FLOATS or (residual is not None and residual.dtype not in _FLOATS):
         raise TypeError("residual and weight must have dtype torch.bfloat16 or torch.float32")
-    tensors = (hidden_states, weight) if residual is None else (hidden_states, weight, residual)
-    device = hidden_states.device
-    if any(t.device != device for t in tensors):
+    device = x.device
+    if weight.device != device or (residual is not None and residual.device != device):
         raise ValueError("all inputs must be on the same device")
-    if any(not t.is_contiguous() for t in tensors):
+    if not x.is_contiguous() or not weight.is_contiguous() or \
+            (residual is not None and not residual.is_contiguous()):
         raise ValueError("all inputs must be contiguous")
-    if any(t.requires_grad for t in tensors):
+    if x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad):
         raise ValueError("the native norm does not support autograd")
     if hidden < 1 or hidden % step or hidden > MAX_NORM_HIDDEN:
         raise ValueError(f"hidden_size must be a multiple of {step} and at most {MAX_NORM_HIDDEN}")
-    if hidden_states.numel() // hidden > 0x7FFFFFFF:
+    rows = x.numel() // hidden
+    if rows > 0x7FFFFFFF:
         raise ValueError("the native norm supports at most 2**31 - 1 rows")
     if device.type != "cuda":
         raise ValueError("the native norm requires CUDA tensors")
+    return rows
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    a0, b0 = a.data_ptr(), b.data_ptr()
-    return a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
+def _launch(x, residual, weight, eps, rows: int, out, scale, residual_out) -> None:
+    """Checks what the results may overlap, and enqueues the kernel.  An output may be the hidden
+    states or the residual themselves (in-place use, same dtype); any other overlap would let one
+    row's stores reach another row's loads."""
 
-
-def _check_aliases(hidden_states, residual, weight, outputs) -> None:
-    """An output may be the hidden states or the residual themselves (in-place use); any other
-    overlap would let one row's stores reach another row's loads."""
-
-    for i, out in enumerate(outputs):
-        for other in outputs[i + 1:]:
-            if _overlap(out, other):
-                raise ValueError("the output tensors must not overlap")
-        if _overlap(out, weight):
-            raise ValueError("the output tensors must not overlap the weight")
-        for t in (hidden_states,) if residual is None else (hidden_states, residual):
-            if _overlap(out, t) and not (out.data_ptr() == t.data_ptr() and out.shape == t.shape
-                                         and out.dtype == t.dtype):
-                raise ValueError("an output may only overlap an input by being that tensor")
-
-
-def _launch(hidden_states, residual, weight, eps, out, codes, scale, residual_out) -> None:
-    rows = hidden_states.numel() // hidden_states.shape[-1]
     if rows == 0:
         return
-    device = hidden_states.device
-    index = device.index
-    args = (
-        hidden_states.data_ptr(),
-        None if residual is None else residual.data_ptr(),
-        residual is not None and residual.dtype is torch.float32,
-        weight.data_ptr(), weight.dtype is torch.float32, rows, hidden_states.shape[-1], eps,
-        None if out is None else out.data_ptr(), None if codes is None else codes.data_ptr(),
-        None if scale is None else scale.data_ptr(),
-        None if residual is None else residual_out.data_ptr(),
-        torch._C._cuda_getCurrentRawStream(index),
-    )
+    hidden = x.shape[-1]
+    count = rows * hidden
+    x_at, w_at, out_at = x.data_ptr(), weight.data_ptr(), out.data_ptr()
+    w_f32 = weight.dtype is torch.float32
+    w_end = w_at + hidden * (4 if w_f32 else 2)
+    out_size = 2 if scale is None else 1
+    # (start, end, element size) of what is read row by row, and of what is written
+    read = [(x_at, x_at + 2 * count, 2)]
+    written = [(out_at, out_at + out_size * count, out_size)]
+    r_at = kept_at = scale_at = None
+    r_f32 = False
+    if residual is not None:
+        r_f32 = residual.dtype is torch.float32
+        size = 4 if r_f32 else 2
+        r_at, kept_at = residual.data_ptr(), residual_out.data_ptr()
+        read.append((r_at, r_at + size * count, size))
+        written.append((kept_at, kept_at + size * count, size))
+    if scale is not None:
+        scale_at = scale.data_ptr()
+        written.append((scale_at, scale_at + 4 * rows, 0))
+    for i, (start, end, size) in enumerate(written):
+        for start2, end2, _ in written[i + 1:]:
+            if start < end2 and start2 < end:
+                raise ValueError("the output tensors must not overlap")
+        if start < w_end and w_at < end:
+            raise ValueError("the output tensors must not overlap the weight")
+        for start2, end2, size2 in read:
+            if start < end2 and start2 < end and (start != start2 or size != size2):
+                raise ValueError("an output may only overlap an input by being that tensor")
+    index = x.device.index
+    args = (x_at, r_at, r_f32, w_at, w_f32, rows, hidden, eps, out_at if scale is None else None,
+            None if scale is None else out_at, scale_at, kept_at,
+            torch._C._cuda_getCurrentRawStream(index))
     fn = _lib.load().b200moe_add_rms_norm
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         code = fn(*args)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             code = fn(*args)
     if code:
         _lib.check(code, "b200moe_add_rms_norm")
 
 
-def _residual_buffer(hidden_states, residual, residual_out):
+def _residual_buffer(residual, residual_out):
     if residual is None:
         if residual_out is not None:
             raise ValueError("residual_out needs a residual")
@@ -148,15 +158,13 @@ def add_rms_norm(
     other overlap is allowed.
     """
 
-    _check(hidden_states, residual, weight, eps, 8)
+    rows = _check(hidden_states, residual, weight, eps, 8)
     if out is None:
         out = torch.empty_like(hidden_states)
     else:
         _check_buffer("out", out, hidden_states.shape, torch.bfloat16, hidden_states.device)
-    residual_out = _residual_buffer(hidden_states, residual, residual_out)
-    _check_aliases(hidden_states, residual, weight,
-                   (out,) if residual is None else (out, residual_out))
-    _launch(hidden_states, residual, weight, eps, out, None, None, residual_out)
+    residual_out = _residual_buffer(residual, residual_out)
+    _launch(hidden_states, residual, weight, eps, rows, out, None, residual_out)
     return out, hidden_states if residual is None else residual_out
 
 
@@ -178,19 +186,16 @@ def add_rms_norm_fp8(
     multiple of 16.
     """
 
-    _check(hidden_states, residual, weight, eps, 16)
+    rows = _check(hidden_states, residual, weight, eps, 16)
+    device = hidden_states.device
     if out is None:
-        out = torch.empty(hidden_states.shape, dtype=torch.uint8, device=hidden_states.device)
+        out = torch.empty(hidden_states.shape, dtype=torch.uint8, device=device)
     else:
-        _check_buffer("out", out, hidden_states.shape, torch.uint8, hidden_states.device)
+        _check_buffer("out", out, hidden_states.shape, torch.uint8, device)
     if scale_out is None:
-        scale_out = torch.empty(hidden_states.shape[:-1], dtype=torch.float32,
-                                device=hidden_states.device)
+        scale_out = torch.empty(hidden_states.shape[:-1], dtype=torch.float32, device=device)
     else:
-        _check_buffer("scale_out", scale_out, hidden_states.shape[:-1], torch.float32,
-                      hidden_states.device)
-    residual_out = _residual_buffer(hidden_states, residual, residual_out)
-    _check_aliases(hidden_states, residual, weight,
-                   (out, scale_out) if residual is None else (out, scale_out, residual_out))
-    _launch(hidden_states, residual, weight, eps, None, out, scale_out, residual_out)
+        _check_buffer("scale_out", scale_out, hidden_states.shape[:-1], torch.float32, device)
+    residual_out = _residual_buffer(residual, residual_out)
+    _launch(hidden_states, residual, weight, eps, rows, out, scale_out, residual_out)
     return out, scale_out, hidden_states if residual is None else residual_out

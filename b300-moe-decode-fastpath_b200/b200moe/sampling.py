@@ -121,7 +121,7 @@ def sample_tokens(
             None if logprobs is None else logprobs.data_ptr(),
             torch._C._cuda_getCurrentRawStream(device.index))
     fn = _lib.load().b200moe_sample
-    if torch.cuda.current_device() == device.index:
+    if torch._C._cuda_getDevice() == device.index:
         code = fn(*args)
     else:
         with torch.cuda.device(device):

@@ -73,6 +73,7 @@ class B300MoEWorkspace:
         self._recorded_streams: set[int] = set()
         self._args_cache: tuple[object, object] | None = None  # bound native argument struct
         self._plan = None  # facts established by the last fully checked forward (forward.py)
+        self._layer_binding = None  # the one-kernel layer's argument struct (layer.py)
         self._lock = threading.RLock()
 
     # -- read-only state --------------------------------------------------------
@@ -230,6 +231,7 @@ class B300MoEWorkspace:
         self._recorded_streams = set()
         self._args_cache = None
         self._plan = None
+        self._layer_binding = None
         if native and device.type == "cuda":
             need = _lib.scratch_bytes(tokens, top_k, num_experts, hidden, inter)
             base = torch.empty(need + _SCRATCH_ALIGN, device=device, dtype=torch.uint8)

@@ -8,6 +8,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/b200moe.h"
 
 namespace b200moe {
@@ -172,6 +174,21 @@ __host__ __device__ inline ScratchLayout scratch_layout(int rows_cap, int expert
   const int few_rows = rows_cap < 8 * kFewMaxTokens ? rows_cap : 8 * kFewMaxTokens;
   l.total = align_up(l.few_acts + (size_t)few_rows * inter * 4, kScratchAlign);
   return l;
+}
+
+// Lets `kernel` ask for all of an SM's shared memory, once per device; `done` is the caller's,
+// one bit per device.  (Two threads that come here first at the same time both ask.)
+constexpr int kMostSharedMemory = 227 * 1024;
+inline cudaError_t allow_shared_memory(const void* kernel, std::atomic<uint64_t>& done) {
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kMostSharedMemory);
+  if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return err;
 }
 
 // ---------------------------------------------------------------------------

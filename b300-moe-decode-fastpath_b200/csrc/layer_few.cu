@@ -916,7 +916,7 @@ struct FewShape {
   size_t bytes;
 };
 bool few_shape(size_t x_bytes, FewShape* shape) {
-  constexpr size_t kMost = 227 * 1024;
+  constexpr size_t kMost = kMostSharedMemory;
   const FewShape options[4] = {{2, 3, 0}, {2, 2, 0}, {1, 3, 0}, {1, 2, 0}};
   for (const FewShape& o : options) {
     const size_t fixed = o.subs == 2 ? sizeof(FewShared<2>) : sizeof(FewShared<1>);
@@ -980,8 +980,9 @@ cudaError_t launch_layer_few(const void* x, const void* router, bool router_f32,
                                          : few_kernel<true, false>(shape))
                            : (router_f32 ? few_kernel<false, true>(shape)
                                          : few_kernel<false, false>(shape));
-  cudaError_t err =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shape.bytes);
+  static std::atomic<uint64_t> allowed[2][2][2][2];
+  cudaError_t err = allow_shared_memory(
+      kernel, allowed[fp8][router_f32][shape.subs - 1][shape.stages - 2]);
   if (err != cudaSuccess) return err;
   void* args[] = {&p};
   return cudaLaunchCooperativeKernel(kernel, dim3(sm_count), dim3(kFewThreads), args, shape.bytes,

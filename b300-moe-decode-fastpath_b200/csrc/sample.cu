@@ -914,8 +914,8 @@ cudaError_t launch_sample(const void* logits, bool logits_f32, long long row_str
   const size_t bytes = sizeof(SampleShared) + (size_t)(p.slice + 3) * sizeof(float);
   const void* kernel = logits_f32 ? (const void*)sample_kernel<float>
                                   : (const void*)sample_kernel<__nv_bfloat16>;
-  cudaError_t err =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  static std::atomic<uint64_t> allowed[2];
+  cudaError_t err = allow_shared_memory(kernel, allowed[logits_f32]);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)rows * blocks);
