@@ -12,7 +12,7 @@
 // threshold on the logit and the index of the last token kept among those equal to it.  A
 // histogram over 2048 bins linear in m - x (for top-k of counts, for top-p of weights) finds the
 // bin in which the wanted sum is crossed; the few hundred tokens of that bin are collected in a
-// list and sorted.  Where top-k leaves few tokens altogether they are collected instead, and one block does the rest.  A bin with more than 1024 tokens
+// list and compared with one another.  Where top-k leaves few tokens altogether they are collected instead, and one block does the rest.  A bin with more than 1024 tokens
 // (equal logits, a range far from that of the weights) is taken apart by three histograms over
 // the digits (11, 11 and 10 bits) of the logit's ordered bit pattern.  A row is read from memory
 // once and stays in the shared memory of a cluster of up to eight blocks, which exchange
@@ -83,7 +83,8 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 // with at most 2^15 tokens in a block their sums stay within 32 bits.
 constexpr int kPartBits = 15;
 constexpr int kGroups = 64;            // groups of 32 bins
-constexpr int kList = 1024;            // tokens that are sorted
+constexpr int kList = 1024;            // tokens of a list
+constexpr int kPairs = 256;            // up to so many are compared with one another, else sorted
 constexpr int kPieces = 256;           // of a bin
 
 struct Found {
@@ -94,7 +95,7 @@ struct Found {
 
 struct alignas(16) SampleShared {
   uint32_t part[3][kBins];     // counts: the first one only
-  uint2 list[kList];           // {key, index}; the cluster's in its first block
+  u64 list[kList];             // of this block: {key, index}
   u64 group[kGroups];          // of this block
   u64 group_total[kGroups];    // of the cluster
   u64 bins[kMaxCluster][32];   // a group of bins of every block
@@ -231,16 +232,19 @@ __device__ __forceinline__ void clear_bins(SampleShared& sh) {
     if (BY_MASS) sh.part[1][b] = sh.part[2][b] = 0u;
   }
 }
-__device__ __forceinline__ void add_mass(SampleShared& sh, int bin, u64 w) {
+// `part`: three arrays of BINS counters, one behind the other
+template <int BINS>
+__device__ __forceinline__ void add_mass(uint32_t* part, int bin, u64 w) {
   constexpr uint32_t mask = (1u << kPartBits) - 1u;
-  atomicAdd(&sh.part[0][bin], (uint32_t)w & mask);
-  atomicAdd(&sh.part[1][bin], (uint32_t)(w >> kPartBits) & mask);
-  atomicAdd(&sh.part[2][bin], (uint32_t)(w >> (2 * kPartBits)));
+  atomicAdd(part + bin, (uint32_t)w & mask);
+  atomicAdd(part + BINS + bin, (uint32_t)(w >> kPartBits) & mask);
+  atomicAdd(part + 2 * BINS + bin, (uint32_t)(w >> (2 * kPartBits)));
 }
-template <bool BY_MASS>
-__device__ __forceinline__ u64 bin_amount(const uint32_t (*part)[kBins], int bin) {
-  u64 v = part[0][bin];
-  if (BY_MASS) v += ((u64)part[1][bin] << kPartBits) + ((u64)part[2][bin] << (2 * kPartBits));
+template <bool BY_MASS, int BINS = kBins>
+__device__ __forceinline__ u64 bin_amount(const uint32_t* part, int bin) {
+  u64 v = part[bin];
+  if (BY_MASS)
+    v += ((u64)part[BINS + bin] << kPartBits) + ((u64)part[2 * BINS + bin] << (2 * kPartBits));
   return v;
 }
 __device__ __forceinline__ u64 inclusive_scan(u64 v) {
@@ -265,7 +269,7 @@ __device__ Found find_bin(SampleShared& sh, cg::cluster_group& cluster, Need nee
     static_assert(kBins == 4 * kSampleThreads && kBins == 32 * kGroups, "bins per thread");
     u64 v = 0ull;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v += bin_amount<BY_MASS>(sh.part, 4 * threadIdx.x + i);
+    for (int i = 0; i < 4; ++i) v += bin_amount<BY_MASS>(sh.part[0], 4 * threadIdx.x + i);
 #pragma unroll
     for (int m = 4; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
     if ((threadIdx.x & 7) == 0) sh.group[threadIdx.x / 8] = v;
@@ -297,7 +301,7 @@ __device__ Found find_bin(SampleShared& sh, cg::cluster_group& cluster, Need nee
   }
   const int bin = group * 32 + lane;
   if (warp < blocks)  // one warp per block of the cluster: a single trip
-    sh.bins[warp][lane] = bin_amount<BY_MASS>(cluster.map_shared_rank(sh.part, warp), bin);
+    sh.bins[warp][lane] = bin_amount<BY_MASS>(cluster.map_shared_rank(sh.part[0], warp), bin);
   __syncthreads();
   if (warp == 0) {
     u64 v = 0ull;
@@ -313,10 +317,13 @@ __device__ Found find_bin(SampleShared& sh, cg::cluster_group& cluster, Need nee
   return sh.found;
 }
 
-// Appends the warp's chosen tokens to the list of the cluster's first block; `count` goes on
-// counting where the list is full.
-__device__ __forceinline__ void append(bool chosen, uint32_t key, int index, uint2* list,
-                                       unsigned* count) {
+// (logit, index) as one integer, in the order of the tokens
+__device__ __forceinline__ u64 place(uint32_t key, int index) { return ((u64)key << 32) | (unsigned)index; }
+__device__ __forceinline__ float logit_at(u64 place) { return logit_of((uint32_t)(place >> 32)); }
+
+// Appends the warp's chosen tokens to the block's list; `count` goes on counting where that is
+// full.
+__device__ __forceinline__ void append(bool chosen, u64 entry, u64* list, unsigned* count) {
   const unsigned votes = __ballot_sync(0xffffffffu, chosen);
   if (votes == 0u) return;
   const int lane = threadIdx.x & 31, leader = __ffs(votes) - 1;
@@ -324,8 +331,64 @@ __device__ __forceinline__ void append(bool chosen, uint32_t key, int index, uin
   if (lane == leader) base = atomicAdd(count, (unsigned)__popc(votes));
   base = __shfl_sync(0xffffffffu, base, leader);
   const unsigned at = base + __popc(votes & ((1u << lane) - 1u));
-  if (chosen && at < (unsigned)kList) list[at] = make_uint2(key, (unsigned)index);
+  if (chosen && at < (unsigned)kList) list[at] = entry;
 }
+// The number of tokens in all lists of the cluster, and, where they fit, a copy of them in
+// `merged`.  The lists have to stay until every block has come past a further cluster barrier.
+__device__ __forceinline__ unsigned merge_lists(SampleShared& sh, cg::cluster_group& cluster,
+                                                unsigned* count, u64* merged) {
+  const unsigned blocks = cluster.num_blocks();
+  unsigned n[kMaxCluster], total = 0u;
+#pragma unroll
+  for (unsigned r = 0; r < kMaxCluster; ++r)
+    n[r] = r < blocks ? *cluster.map_shared_rank(count, r) : 0u;
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; ++r) total += n[r];
+  if (merged && total <= (unsigned)kList) {
+    unsigned at = 0u;
+#pragma unroll
+    for (unsigned r = 0; r < kMaxCluster; ++r) {
+      if (r < blocks)
+        for (unsigned i = threadIdx.x; i < n[r]; i += kSampleThreads)
+          merged[at + i] = cluster.map_shared_rank(sh.list, r)[i];
+      at += n[r];
+    }
+  }
+  return total;
+}
+
+// For n <= kPairs entries in shared memory: of the entry that this thread shares with its
+// neighbours (`lanes` of them), how many come before it, and the sum of their weights.
+struct Before {
+  int entry;     // -1: none
+  bool first;    // of the threads that share it
+  int rank;
+  u64 sum;
+};
+__device__ __forceinline__ Before compare_all(const u64* entry, const u64* weight, int n) {
+  const int padded = n <= 1 ? 1 : 1 << (32 - __clz(n - 1));
+  const int lanes = min(32, kSampleThreads / padded), part = threadIdx.x & (lanes - 1);
+  Before b;
+  b.entry = threadIdx.x / lanes;
+  b.first = part == 0;
+  b.rank = 0;
+  b.sum = 0ull;
+  const bool in = b.entry < n;
+  const u64 mine = in ? entry[b.entry] : 0ull;
+#pragma unroll 2
+  for (int j = part; j < n; j += lanes)
+    if (entry[j] < mine) {
+      ++b.rank;
+      b.sum += weight[j];
+    }
+  for (int m = lanes >> 1; m > 0; m >>= 1) {
+    b.rank += __shfl_xor_sync(0xffffffffu, b.rank, m);
+    b.sum += __shfl_xor_sync(0xffffffffu, b.sum, m);
+  }
+  if (!in) b.entry = -1;
+  return b;
+}
+
 // Sorts `count` integers, two per thread (2 t and 2 t + 1), ascending; what is behind them must be
 // ~0.  A bitonic network: partners within a warp exchange by shuffles, others through `scratch`
 // (two integers per thread).  Threads without a share only keep the barriers.
@@ -384,9 +447,6 @@ __device__ __forceinline__ u64 block_scan(SampleShared& sh, u64 v, u64& total) {
   }
   return before + upto - v;
 }
-// (logit, index) as one integer, in the order of the tokens
-__device__ __forceinline__ u64 place(const uint2& e) { return ((u64)e.x << 32) | e.y; }
-
 // The shortest prefix of the kept tokens whose sum (of counts, or of weights) ends in bin
 // `found.bin` of the linear histogram, `rest` (at least 1) into it.
 template <bool BY_MASS>
@@ -395,8 +455,7 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int from = warp * row.chunk, to = min(row.n, from + row.chunk);
   // the bin's tokens
-  uint2* list = cluster.map_shared_rank(sh.list, 0);
-  unsigned* count = cluster.map_shared_rank(&sh.list_n[BY_MASS], 0);
+  unsigned* count = &sh.list_n[BY_MASS];
   for (int i = from + lane; i - lane < to; i += 32 * kWide) {
     float v[kWide];
     bool chosen[kWide], any = false;
@@ -411,21 +470,23 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
     for (int j = 0; j < kWide; ++j) {
       const uint32_t key = descending_key(v[j]);
       const int index = row.base + i + 32 * j;
-      append(chosen[j] && kept.holds(key, index), key, index, list, count);
+      append(chosen[j] && kept.holds(key, index), place(key, index), sh.list, count);
     }
   }
-  cluster.sync();
-  const unsigned n = *count;
+  cluster.sync();  // the lists are complete, and the histogram has been read
+  u64* merged = reinterpret_cast<u64*>(&sh.part[2][0]);  // the pieces are in part[0] and part[1]
+  const unsigned n = merge_lists(sh, cluster, count, merged);
   Kept next;
   if (n <= (unsigned)kList) {
     // A histogram of the list over 256 pieces of the bin narrows it down to the tokens of one
     // piece, mostly one or two; those are sorted.  Every block does this for itself.
     static_assert(kList <= 2 * kSampleThreads, "two tokens per thread");
-    if (threadIdx.x < kPieces) sh.part[0][threadIdx.x] = sh.part[1][threadIdx.x] = sh.part[2][threadIdx.x] = 0u;
+    static_assert(3 * kPieces <= kBins, "the three parts of the pieces fit part[0]");
+    uint32_t* pieces = sh.part[0];
+    for (int i = threadIdx.x; i < 3 * kPieces; i += kSampleThreads) pieces[i] = 0u;
     if (threadIdx.x == 0) sh.piece_n = 0u;
     __syncthreads();
-    uint2 e[2];
-    u64 w[2];
+    u64 e[2], w[2];
     int piece[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -433,18 +494,18 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
       w[q] = 0ull;
       piece[q] = -1;
       if (i >= n) continue;
-      e[q] = list[i];
-      const float v = logit_of(e[q].x);
+      e[q] = merged[i];
+      const float v = logit_at(e[q]);
       w[q] = BY_MASS ? weigh(v) : 1ull;
       piece[q] = row.piece(v, bin);
-      if (w[q]) add_mass(sh, piece[q], w[q]);
+      if (w[q]) add_mass<kPieces>(pieces, piece[q], w[q]);
     }
     __syncthreads();
     // every warp: eight pieces per lane
     u64 amount[kPieces / 32], sum = 0ull;
 #pragma unroll
     for (int i = 0; i < kPieces / 32; ++i) {
-      amount[i] = bin_amount<true>(sh.part, lane * (kPieces / 32) + i);
+      amount[i] = bin_amount<true, kPieces>(pieces, lane * (kPieces / 32) + i);
       sum += amount[i];
     }
     u64 run = inclusive_scan(sum) - sum;
@@ -460,30 +521,39 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
     const int at = __ffs(__ballot_sync(0xffffffffu, mine >= 0)) - 1;
     mine = __shfl_sync(0xffffffffu, mine, at);
     rest -= __shfl_sync(0xffffffffu, run, at);
-    u64* some = reinterpret_cast<u64*>(&sh.part[1][0]);  // behind the pieces of part[0], and in
-    __syncthreads();                                     // place of the others
+    u64* some = reinterpret_cast<u64*>(&sh.part[1][0]);
 #pragma unroll
     for (int q = 0; q < 2; ++q)
-      if (piece[q] == mine) some[atomicAdd(&sh.piece_n, 1u)] = place(e[q]);
+      if (piece[q] == mine) some[atomicAdd(&sh.piece_n, 1u)] = e[q];
     __syncthreads();
     const int m = (int)sh.piece_n;
-    u64 v[2], total;
+    if (m <= kPairs) {
+      u64* weight = some + kPairs;
+      if (threadIdx.x < m) weight[threadIdx.x] = BY_MASS ? weigh(logit_at(some[threadIdx.x])) : 1ull;
+      __syncthreads();
+      const Before b = compare_all(some, weight, m);
+      if (b.entry >= 0 && b.first && b.sum < rest && b.sum + weight[b.entry] >= rest) {
+        sh.kept_key = (uint32_t)(some[b.entry] >> 32);
+        sh.kept_last = (int)(uint32_t)some[b.entry];
+      }
+    } else {
+      u64 v[2], total;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) v[q] = 2 * threadIdx.x + q < m ? some[2 * threadIdx.x + q] : ~0ull;
-    sort_block(v, m, reinterpret_cast<ulonglong2*>(&sh.part[1][0]));
+      for (int q = 0; q < 2; ++q) v[q] = 2 * threadIdx.x + q < m ? some[2 * threadIdx.x + q] : ~0ull;
+      sort_block(v, m, reinterpret_cast<ulonglong2*>(&sh.part[1][0]));
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
-      w[q] = v[q] == ~0ull ? 0ull : BY_MASS ? weigh(logit_of((uint32_t)(v[q] >> 32))) : 1ull;
-    const u64 before = block_scan(sh, w[0] + w[1], total);
-    if (before < rest && before + w[0] + w[1] >= rest) {
-      const u64 last = before + w[0] >= rest ? v[0] : v[1];
-      sh.kept_key = (uint32_t)(last >> 32);
-      sh.kept_last = (int)(uint32_t)last;
+      for (int q = 0; q < 2; ++q) w[q] = v[q] == ~0ull ? 0ull : BY_MASS ? weigh(logit_at(v[q])) : 1ull;
+      const u64 before = block_scan(sh, w[0] + w[1], total);
+      if (before < rest && before + w[0] + w[1] >= rest) {
+        const u64 last = before + w[0] >= rest ? v[0] : v[1];
+        sh.kept_key = (uint32_t)(last >> 32);
+        sh.kept_last = (int)(uint32_t)last;
+      }
     }
     __syncthreads();
     next.key = sh.kept_key;
     next.last = sh.kept_last;
-    cluster.sync();  // the first block's list has been read
+    cluster.sync();  // the lists have been read
     return next;
   }
 
@@ -502,7 +572,7 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
       const uint32_t key = descending_key(v);
       if (row.bin(v) != bin || (key & mask) != prefix || !kept.holds(key, row.base + i)) continue;
       const int digit = (key >> shift) & digits;
-      if (BY_MASS) add_mass(sh, digit, weigh(v));
+      if (BY_MASS) add_mass<kBins>(sh.part[0], digit, weigh(v));
       else atomicAdd(&sh.part[0][digit], 1u);
     }
     u64 total;
@@ -574,20 +644,55 @@ __device__ __forceinline__ void store_result(const SampleParams& p, int row_id,
                                  (log((double)total) - kWeightBits * 0.69314718055994530942));
 }
 
-// All that is left after top-k fits the list: one block sorts it, cuts it to k tokens, weighs them,
-// cuts to top-p, and sorts what is left by index for the draw.
+// All that is left after top-k fits a list (in part[2]): one block cuts it to k tokens, weighs
+// them, cuts to top-p and draws.  A short list is compared entry by entry, a long one sorted by
+// the order and, for the draw, by index.
 __device__ void finish_list(SampleShared& sh, const SampleParams& p, int row_id,
-                            const Weigher& weigh, int top_k, float top_p, float u) {
-  const int n = (int)sh.list_n[0], at = 2 * threadIdx.x;
+                            const Weigher& weigh, u64* entry, int n, int top_k, float top_p,
+                            float u) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 total;
+  __syncthreads();
+  if (n <= kPairs) {
+    u64* weight = reinterpret_cast<u64*>(&sh.part[0][0]);
+    if (threadIdx.x < n) weight[threadIdx.x] = weigh(logit_at(entry[threadIdx.x]));
+    __syncthreads();
+    const Before b = compare_all(entry, weight, n);
+    const bool mine = b.entry >= 0 && b.first;
+    u64 w = mine && b.rank < top_k ? weight[b.entry] : 0ull;
+    u64 sum = warp_total(w);
+    if (lane == 0) sh.warp_sum[warp] = sum;
+    total = block_total(sh);  // and all weights have been read
+    if (top_p < 1.0f) {
+      if (b.sum >= mass_needed(top_p, total)) w = 0ull;
+      sum = warp_total(w);
+      __syncthreads();
+      if (lane == 0) sh.warp_sum[warp] = sum;
+      total = block_total(sh);
+    }
+    // again by index; {index, key}
+    u64* by_index = reinterpret_cast<u64*>(&sh.part[1][0]);
+    if (mine) {
+      weight[b.entry] = w;
+      by_index[b.entry] = (entry[b.entry] << 32) | (entry[b.entry] >> 32);
+    }
+    __syncthreads();
+    const Before d = compare_all(by_index, weight, n);
+    const u64 target = draw_target(u, total);
+    if (d.entry >= 0 && d.first && d.sum <= target && target < d.sum + weight[d.entry])
+      store_result(p, row_id, weigh, (int)(uint32_t)entry[d.entry], logit_at(entry[d.entry]), total);
+    return;
+  }
+  const int at = 2 * threadIdx.x;
   ulonglong2* scratch = reinterpret_cast<ulonglong2*>(&sh.part[0][0]);
-  u64* entry = reinterpret_cast<u64*>(&sh.part[2][0]);
-  u64 v[2], w[2], total;
+  u64 v[2], w[2];
 #pragma unroll
-  for (int q = 0; q < 2; ++q) v[q] = at + q < n ? place(sh.list[at + q]) : ~0ull;
+  for (int q = 0; q < 2; ++q) v[q] = at + q < n ? entry[at + q] : ~0ull;
+  __syncthreads();
   sort_block(v, n, scratch);
 #pragma unroll
   for (int q = 0; q < 2; ++q)
-    w[q] = at + q < n && at + q < top_k ? weigh(logit_of((uint32_t)(v[q] >> 32))) : 0ull;
+    w[q] = at + q < n && at + q < top_k ? weigh(logit_at(v[q])) : 0ull;
   u64 before = block_scan(sh, w[0] + w[1], total);
   if (top_p < 1.0f) {
     const u64 need = mass_needed(top_p, total);
@@ -607,7 +712,7 @@ __device__ void finish_list(SampleShared& sh, const SampleParams& p, int row_id,
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const u64 e = v[q] != ~0ull ? entry[(unsigned)v[q]] : 0ull;
-    x[q] = logit_of((uint32_t)(e >> 32));
+    x[q] = logit_at(e);
     index[q] = (int)(uint32_t)e;
     w[q] = v[q] != ~0ull ? weigh(x[q]) : 0ull;
   }
@@ -754,12 +859,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   const int from = warp * row.chunk, to = min(row.n, from + row.chunk);
   if (top_k > 0 && top_k < p.vocab) {
     unsigned beyond = 0u;  // in the last bin, where most tokens are: counted apart
-    for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
-      const float v = x[i];
-      if (v == -INFINITY) continue;
-      const int b = row.bin(v);
-      if (b == kBins - 1) ++beyond;
-      else atomicAdd(&sh.part[0][b], 1u);
+    for (int i = from + lane; i < to; i += 32 * kWide) {
+      float v[kWide];
+#pragma unroll
+      for (int j = 0; j < kWide; ++j) v[j] = i + 32 * j < to ? x[i + 32 * j] : -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kWide; ++j) {
+        const int b = row.bin(v[j]);
+        if (v[j] == -INFINITY) continue;
+        if (b == kBins - 1) ++beyond;
+        else atomicAdd(&sh.part[0][b], 1u);
+      }
     }
     beyond = __reduce_add_sync(0xffffffffu, beyond);
     if (lane == 0 && beyond) atomicAdd(&sh.part[0][kBins - 1], beyond);
@@ -768,8 +878,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     if (found.bin >= 0 && live > (u64)top_k) {
       if (found.before + found.amount <= (u64)kList) {
         // all tokens up to the end of this bin: the first block of the cluster goes on alone
-        uint2* list = cluster.map_shared_rank(sh.list, 0);
-        unsigned* count = cluster.map_shared_rank(&sh.list_n[0], 0);
         for (int i = from + lane; i - lane < to; i += 32 * kWide) {
           float v[kWide];
           bool chosen[kWide], any = false;
@@ -782,10 +890,18 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
           if (!__any_sync(0xffffffffu, any)) continue;
 #pragma unroll
           for (int j = 0; j < kWide; ++j)
-            append(chosen[j], descending_key(v[j]), row.base + i + 32 * j, list, count);
+            append(chosen[j], place(descending_key(v[j]), row.base + i + 32 * j), sh.list,
+                   &sh.list_n[0]);
         }
-        cluster.sync();
-        if (rank == 0) finish_list(sh, p, row_id, weigh, top_k, top_p, u);
+        cluster.sync();  // the lists are complete, and the histogram has been read
+        u64* merged = reinterpret_cast<u64*>(&sh.part[2][0]);
+        if (rank == 0) {
+          const int n = (int)merge_lists(sh, cluster, &sh.list_n[0], merged);
+          cluster.sync();
+          finish_list(sh, p, row_id, weigh, merged, n, top_k, top_p, u);
+        } else {
+          cluster.sync();  // no block leaves while another reads its shared memory
+        }
         return;
       }
       kept = select<false>(sh, cluster, row, weigh, kept, found.bin, (u64)top_k - found.before);
@@ -818,7 +934,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     if (nucleus) {
 #pragma unroll
       for (int j = 0; j < kWide; ++j)
-        if (w[j]) add_mass(sh, row.bin(v[j]), w[j]);
+        if (w[j]) add_mass<kBins>(sh.part[0], row.bin(v[j]), w[j]);
     }
   }
   u64 total = 0ull;
