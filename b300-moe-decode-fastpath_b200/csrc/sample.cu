@@ -35,6 +35,7 @@
 // branches: one after the other, each waiting for twelve dependent FP64 operations, they took
 // 15 us for 16,160 tokens of a block.
 #include <cooperative_groups.h>
+#include <float.h>
 
 #include "common.cuh"
 
@@ -52,7 +53,15 @@ constexpr int kWeightBits = 45;
 constexpr int kPowers = 128;
 constexpr int kMaxCluster = 8;
 constexpr int kWide = 4;      // tokens that a thread weighs at a time
-constexpr uint32_t kMinusInfKey = 0xFF800000u;  // descending_key(-inf)
+constexpr int kPad = kSampleThreads * kWide;
+
+// Weights are added up in the histogram as three parts of 15 bits (the highest may be 2^15):
+// with at most 2^15 tokens in a block their sums stay within 32 bits.
+constexpr int kPartBits = 15;
+constexpr int kGroups = 64;            // groups of 32 bins
+constexpr int kList = 1024;            // tokens of a list
+constexpr int kPairs = 256;            // up to so many are compared with one another, else sorted
+constexpr int kPieces = 256;           // of a bin
 
 struct SampleParams {
   const void* logits;
@@ -79,14 +88,6 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key : ~key & 0x7FFFFFFFu);
 }
 
-// Weights are added up in the histogram as three parts of 15 bits (the highest may be 2^15):
-// with at most 2^15 tokens in a block their sums stay within 32 bits.
-constexpr int kPartBits = 15;
-constexpr int kGroups = 64;            // groups of 32 bins
-constexpr int kList = 1024;            // tokens of a list
-constexpr int kPairs = 256;            // up to so many are compared with one another, else sorted
-constexpr int kPieces = 256;           // of a bin
-
 struct Found {
   int bin;      // -1: the whole histogram stays below what was asked for
   u64 before;   // sum of the bins before it
@@ -109,7 +110,7 @@ struct alignas(16) SampleShared {
   float warp_best[kSampleWarps];
   int warp_first[kSampleWarps];
   unsigned piece_n;
-  uint32_t kept_key;
+  float kept_x;
   int kept_last;
 };
 
@@ -120,6 +121,7 @@ struct Weigher {
   float best_f;
   float lowest;          // a logit whose weight rounds to zero (then also that of all below it)
   bool bounded;          // there is such a logit, and the largest one is finite
+  bool has_least;
   double least;          // min-p: smaller weights are dropped
 
   __device__ __forceinline__ void set(const double* power_, float best_, float temperature,
@@ -131,14 +133,15 @@ struct Weigher {
     lowest = best_ - 40.0f * temperature;  // 2^-57.7
     bounded = isfinite(best_) && isfinite(lowest) && ((double)lowest - best) * rate < -48.0;
     // min-p in units of 2^-45, not above the largest weight; NaN: off
-    least = min_p > 0.0f ? ldexp((double)fminf(min_p, 1.0f), kWeightBits) : 0.0;
+    has_least = min_p > 0.0f;
+    least = has_least ? ldexp((double)fminf(min_p, 1.0f), kWeightBits) : 0.0;
   }
-  // y > -1000
-  __device__ __forceinline__ u64 power_of(double y) const {
+  // y > -1000; k: y in units of 2^-7, rounded
+  __device__ __forceinline__ u64 power_of(double y, int& k) const {
     // y = k / 128 + r: adding 1.5 * 2^45 leaves k in the low bits of the sum
     const double magic = 52776558133248.0;
     const double shifted = y + magic;
-    const int k = __double2loint(shifted);
+    k = __double2loint(shifted);
     const double r = y - (shifted - magic);
     // 2^r = 1 + r (c1 + r (c2 + r (c3 + r c4))), cn = ln(2)^n / n!
     constexpr double c1 = 0.69314718055994530942;
@@ -153,33 +156,60 @@ struct Weigher {
         __double2hiint(v) + (int)(((unsigned)k & ~(unsigned)(kPowers - 1)) << 13), __double2loint(v));
     // round to an integer in the low bits: w <= 2^45
     const u64 n = (u64)__double_as_longlong(w + 4503599627370496.0) & ((1ull << 52) - 1ull);
-    return least > 0.0 && w < least ? 0ull : n;
+    return has_least && w < least ? 0ull : n;
   }
   __device__ __forceinline__ double exponent(float x) const {
     return x == best_f ? 0.0 : ((double)x - best) * rate;
   }
-  // any logit but NaN; -inf: 0
+  // any logit but NaN; -inf: 0.  bin: of the weight histogram, four units of 2^-7 octaves each
+  __device__ __forceinline__ u64 operator()(float x, int& bin) const {
+    int k;
+    u64 w;
+    if (bounded) {
+      w = power_of(((double)fmaxf(x, lowest) - best) * rate, k);
+    } else {
+      const double y = exponent(x);
+      const bool counts = x != -INFINITY && y > -48.0;
+      w = power_of(counts ? y : 0.0, k);
+      if (!counts) w = 0ull;
+    }
+    bin = -k >> 2;  // below 2048: y is above -58
+    return w;
+  }
   __device__ __forceinline__ u64 operator()(float x) const {
-    if (bounded) return power_of(((double)fmaxf(x, lowest) - best) * rate);
-    const double y = exponent(x);
-    return x != -INFINITY && y > -48.0 ? power_of(y) : 0ull;
+    int bin;
+    return (*this)(x, bin);
+  }
+  // A range of logits that holds all of a bin's (and a few of its neighbours').
+  __device__ __forceinline__ void range_of(int bin, float& low, float& high) const {
+    low = -INFINITY;
+    high = INFINITY;
+    if (!bounded) return;
+    const double a = best - (4 * bin + 3.5) / (128.0 * rate), b = best - (4 * bin - 0.5) / (128.0 * rate);
+    low = (float)(a - 1e-6 * fabs(a) - 1e-37);
+    high = (float)(b + 1e-6 * fabs(b) + 1e-37);
+  }
+  // the part of the bin that x lies in, of kPieces
+  __device__ __forceinline__ int piece(float x, int bin) const {
+    const double t = (-128.0 * exponent(x) - (4 * bin - 0.5)) * (kPieces / 4);
+    return (int)fmin(fmax(t, 0.0), (double)(kPieces - 1));
   }
 };
 
-// The tokens kept so far: those that come before (key, index) in the order, or are it.
+// The tokens kept so far: those with a larger logit, and up to index `last` those with this one.
 struct Kept {
-  uint32_t key;
+  float x;
   int last;
-  __device__ __forceinline__ bool holds(uint32_t k, int index) const {
-    return k < key || (k == key && index <= last);
+  __device__ __forceinline__ bool holds(float v, int index) const {
+    return v > x || (v == x && index <= last);
   }
 };
 
 struct Row {
-  const float* x;      // this block's tokens in shared memory
+  const float* x;      // this block's tokens in shared memory, -inf behind them
   int n, base;         // how many, and the index of the first
-  int chunk;           // tokens of a warp, consecutive
-  float best, scale;   // linear bins: (best - x) * scale
+  int chunk;           // tokens of a warp, consecutive; a multiple of 32 kWide
+  float best, scale;   // bins of the count histogram: linear, (best - x) * scale
   __device__ __forceinline__ int bin(float v) const {
     return v == best ? 0 : min(kBins - 1, (int)((best - v) * scale));
   }
@@ -205,6 +235,16 @@ __device__ __forceinline__ u64 warp_total(u64 v) {
   return v;
 }
 
+__device__ __forceinline__ u64 inclusive_scan(u64 v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const u64 o = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
 // Sum over the block of one value per warp (already in sh.warp_sum).
 __device__ __forceinline__ u64 block_total(SampleShared& sh) {
   __syncthreads();
@@ -213,16 +253,22 @@ __device__ __forceinline__ u64 block_total(SampleShared& sh) {
   for (int i = 0; i < kSampleWarps; ++i) s += sh.warp_sum[i];
   return s;
 }
-// The same over the cluster; sh.sum keeps the block's own share.
-__device__ __forceinline__ u64 cluster_total(SampleShared& sh, cg::cluster_group& cluster) {
+// The value that every block of the cluster holds at `p`, one block per lane (0 in other lanes).
+template <typename V>
+__device__ __forceinline__ V cluster_read(cg::cluster_group& cluster, V* p) {
+  const unsigned lane = threadIdx.x & 31;
+  return lane < cluster.num_blocks() ? *cluster.map_shared_rank(p, lane) : V(0);
+}
+// The same over the cluster; sh.sum keeps the block's own share, before: that of the blocks in
+// front of it.
+__device__ __forceinline__ u64 cluster_total(SampleShared& sh, cg::cluster_group& cluster,
+                                             u64& before) {
   const u64 mine = block_total(sh);
   if (threadIdx.x == 0) sh.sum = mine;
   cluster.sync();
-  u64 s = 0ull;
-#pragma unroll
-  for (unsigned r = 0; r < kMaxCluster; ++r)
-    if (r < cluster.num_blocks()) s += *cluster.map_shared_rank(&sh.sum, r);
-  return s;
+  const u64 upto = inclusive_scan(cluster_read(cluster, &sh.sum));
+  before = __shfl_sync(0xffffffffu, upto, (int)cluster.block_rank()) - mine;
+  return __shfl_sync(0xffffffffu, upto, 31);
 }
 
 template <bool BY_MASS>
@@ -247,16 +293,6 @@ __device__ __forceinline__ u64 bin_amount(const uint32_t* part, int bin) {
     v += ((u64)part[BINS + bin] << kPartBits) + ((u64)part[2 * BINS + bin] << (2 * kPartBits));
   return v;
 }
-__device__ __forceinline__ u64 inclusive_scan(u64 v) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const u64 o = __shfl_up_sync(0xffffffffu, v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
-}
-
 // The bin of the cluster's histogram in which the running sum reaches need(total), and the
 // histogram's total.  Every block finds it for itself: from the sums of 64 groups of 32 bins of
 // all blocks, then from the bins of one group.
@@ -339,11 +375,12 @@ __device__ __forceinline__ unsigned merge_lists(SampleShared& sh, cg::cluster_gr
                                                 unsigned* count, u64* merged) {
   const unsigned blocks = cluster.num_blocks();
   unsigned n[kMaxCluster], total = 0u;
+  const unsigned held = cluster_read(cluster, count);
 #pragma unroll
-  for (unsigned r = 0; r < kMaxCluster; ++r)
-    n[r] = r < blocks ? *cluster.map_shared_rank(count, r) : 0u;
-#pragma unroll
-  for (int r = 0; r < kMaxCluster; ++r) total += n[r];
+  for (int r = 0; r < kMaxCluster; ++r) {
+    n[r] = __shfl_sync(0xffffffffu, held, r);
+    total += n[r];
+  }
   if (merged && total <= (unsigned)kList) {
     unsigned at = 0u;
 #pragma unroll
@@ -456,21 +493,26 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
   const int from = warp * row.chunk, to = min(row.n, from + row.chunk);
   // the bin's tokens
   unsigned* count = &sh.list_n[BY_MASS];
-  for (int i = from + lane; i - lane < to; i += 32 * kWide) {
+  float low, high;
+  if (BY_MASS) weigh.range_of(bin, low, high);
+  for (int i = from + lane; i < from + row.chunk; i += 32 * kWide) {
     float v[kWide];
     bool chosen[kWide], any = false;
 #pragma unroll
     for (int j = 0; j < kWide; ++j) {
-      v[j] = i + 32 * j < to ? row.x[i + 32 * j] : -INFINITY;
-      chosen[j] = v[j] != -INFINITY && row.in_bin(v[j], bin);
+      v[j] = row.x[i + 32 * j];
+      chosen[j] = v[j] != -INFINITY && (BY_MASS ? v[j] >= low && v[j] <= high : row.in_bin(v[j], bin));
       any |= chosen[j];
     }
     if (!__any_sync(0xffffffffu, any)) continue;
 #pragma unroll
     for (int j = 0; j < kWide; ++j) {
-      const uint32_t key = descending_key(v[j]);
       const int index = row.base + i + 32 * j;
-      append(chosen[j] && kept.holds(key, index), place(key, index), sh.list, count);
+      if (BY_MASS && chosen[j]) {  // a neighbour of the bin, or dropped by min-p?
+        int b;
+        chosen[j] = weigh(v[j], b) != 0ull && b == bin;
+      }
+      append(chosen[j] && kept.holds(v[j], index), place(descending_key(v[j]), index), sh.list, count);
     }
   }
   cluster.sync();  // the lists are complete, and the histogram has been read
@@ -497,7 +539,7 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
       e[q] = merged[i];
       const float v = logit_at(e[q]);
       w[q] = BY_MASS ? weigh(v) : 1ull;
-      piece[q] = row.piece(v, bin);
+      piece[q] = BY_MASS ? weigh.piece(v, bin) : row.piece(v, bin);
       if (w[q]) add_mass<kPieces>(pieces, piece[q], w[q]);
     }
     __syncthreads();
@@ -533,7 +575,7 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
       __syncthreads();
       const Before b = compare_all(some, weight, m);
       if (b.entry >= 0 && b.first && b.sum < rest && b.sum + weight[b.entry] >= rest) {
-        sh.kept_key = (uint32_t)(some[b.entry] >> 32);
+        sh.kept_x = logit_at(some[b.entry]);
         sh.kept_last = (int)(uint32_t)some[b.entry];
       }
     } else {
@@ -546,12 +588,12 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
       const u64 before = block_scan(sh, w[0] + w[1], total);
       if (before < rest && before + w[0] + w[1] >= rest) {
         const u64 last = before + w[0] >= rest ? v[0] : v[1];
-        sh.kept_key = (uint32_t)(last >> 32);
+        sh.kept_x = logit_at(last);
         sh.kept_last = (int)(uint32_t)last;
       }
     }
     __syncthreads();
-    next.key = sh.kept_key;
+    next.x = sh.kept_x;
     next.last = sh.kept_last;
     cluster.sync();  // the lists have been read
     return next;
@@ -570,10 +612,15 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
     for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
       const float v = row.x[i];
       const uint32_t key = descending_key(v);
-      if (row.bin(v) != bin || (key & mask) != prefix || !kept.holds(key, row.base + i)) continue;
+      if ((key & mask) != prefix || !kept.holds(v, row.base + i)) continue;
       const int digit = (key >> shift) & digits;
-      if (BY_MASS) add_mass<kBins>(sh.part[0], digit, weigh(v));
-      else atomicAdd(&sh.part[0][digit], 1u);
+      if (BY_MASS) {
+        int b;
+        const u64 w = weigh(v, b);
+        if (w && b == bin) add_mass<kBins>(sh.part[0], digit, w);
+      } else if (row.bin(v) == bin) {
+        atomicAdd(&sh.part[0][digit], 1u);
+      }
     }
     u64 total;
     found = find_bin<BY_MASS>(sh, cluster, [&](u64) { return rest; }, total);
@@ -585,28 +632,27 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
   const u64 each = BY_MASS ? weigh(logit_of(prefix)) : 1ull;
   const u64 equal = found.amount / each;
   const u64 ties = (rest + each - 1ull) / each;
-  next.key = prefix;
+  next.x = logit_of(prefix);
   next.last = 0x7FFFFFFF;
   if (ties >= equal) {
-    if (prefix == kept.key) next.last = kept.last;
+    if (next.x == kept.x) next.last = kept.last;
     cluster.sync();  // the histogram has been read
     return next;
   }
   // the index of the ties-th of them
   unsigned hits = 0u;
   for (int i = from + lane; i < to; i += 32)
-    hits += descending_key(row.x[i]) == prefix && kept.holds(prefix, row.base + i);
+    hits += row.x[i] == next.x && kept.holds(next.x, row.base + i);
   hits = __reduce_add_sync(0xffffffffu, hits);
   if (lane == 0) sh.warp_sum[warp] = hits;
   if (threadIdx.x == 0) sh.first = -1;
-  cluster_total(sh, cluster);
-  u64 before = 0ull;
-  for (unsigned r = 0; r < cluster.block_rank(); ++r) before += *cluster.map_shared_rank(&sh.sum, r);
+  u64 before;
+  cluster_total(sh, cluster, before);
   for (int i = 0; i < warp; ++i) before += sh.warp_sum[i];
   if (before < ties && before + hits >= ties) {  // in this warp's tokens
     for (int i = from; i < to; i += 32) {
-      const bool hit = i + lane < to && descending_key(row.x[i + lane]) == prefix &&
-                       kept.holds(prefix, row.base + i + lane);
+      const bool hit = i + lane < to && row.x[i + lane] == next.x &&
+                       kept.holds(next.x, row.base + i + lane);
       const unsigned votes = __ballot_sync(0xffffffffu, hit);
       const unsigned want = (unsigned)(ties - before);  // >= 1
       if ((unsigned)__popc(votes) >= want) {
@@ -624,6 +670,37 @@ __device__ Kept select(SampleShared& sh, cg::cluster_group& cluster, const Row& 
   }
   cluster.sync();
   return next;
+}
+
+// The weights of the kept tokens among the warp's, summed over its lanes' shares.  The kept ones
+// are packed, so that a warp weighs 32 of them at a time however few there are (top-p 0.9 of
+// 129280 tokens keeps about one in ten: 5.8 us of a block when every token is weighed).
+__device__ __forceinline__ u64 sum_kept(SampleShared& sh, const Row& row, const Weigher& weigh,
+                                        const Kept kept) {
+  constexpr int kRoom = 32 * (kWide + 1);
+  static_assert(kSampleWarps * kRoom <= 3 * kBins, "the packed logits lie where the histogram was");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, from = warp * row.chunk;
+  float* packed = reinterpret_cast<float*>(&sh.part[0][0]) + warp * kRoom;
+  int held = 0;
+  u64 sum = 0ull;
+  for (int i = from + lane; i < from + row.chunk; i += 32 * kWide) {
+#pragma unroll
+    for (int j = 0; j < kWide; ++j) {
+      const float v = row.x[i + 32 * j];
+      const bool wanted = kept.holds(v, row.base + i + 32 * j);
+      const unsigned votes = __ballot_sync(0xffffffffu, wanted);
+      if (wanted) packed[held + __popc(votes & ((1u << lane) - 1u))] = v;
+      held += __popc(votes);
+    }
+    __syncwarp();
+    while (held >= 32) {
+      held -= 32;
+      sum += weigh(packed[held + lane]);
+    }
+    __syncwarp();
+  }
+  if (lane < held) sum += weigh(packed[lane]);
+  return sum;
 }
 
 // Top-p's share of a sum of weights, at least 1.
@@ -789,7 +866,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   Row row;
   row.base = min(p.vocab, rank * p.slice);
   row.n = min(p.vocab - row.base, p.slice);
-  row.chunk = (row.n + 32 * kSampleWarps - 1) / (32 * kSampleWarps) * 32;
+  row.chunk = (row.n + kPad - 1) / kPad * (kPad / kSampleWarps);
 
   const float temperature = p.temperature ? __ldg(p.temperature + row_id) : p.temperature_v;
   const int top_k = p.top_k ? __ldg(p.top_k + row_id) : p.top_k_v;
@@ -805,6 +882,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   if (threadIdx.x < kPowers) sh.power[threadIdx.x] = exp2((double)threadIdx.x / kPowers + kWeightBits);
   if (threadIdx.x < 2) sh.list_n[threadIdx.x] = 0u;
   float best = load_row<T>(src, row.n, x);
+  for (int i = row.n + threadIdx.x; i < row.chunk * kSampleWarps; i += kSampleThreads) x[i] = -INFINITY;
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, m));
   if (lane == 0) sh.warp_best[warp] = best;
@@ -814,10 +892,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     sh.best = best;
   }
   cluster.sync();
-  best = -INFINITY;
+  best = lane < blocks ? *cluster.map_shared_rank(&sh.best, lane) : -INFINITY;
 #pragma unroll
-  for (int r = 0; r < kMaxCluster; ++r)
-    if (r < blocks) best = fmaxf(best, *cluster.map_shared_rank(&sh.best, r));
+  for (int m = 4; m > 0; m >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, m));
+  best = __shfl_sync(0xffffffffu, best, 0);
   row.best = best;
 
   if (best == -INFINITY || !(temperature > 0.0f)) {  // nothing to draw, or nothing to draw by
@@ -851,18 +929,18 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   row.scale = fminf((float)(2047.0 / 32.3) / temperature, 3.0e38f);
 
   Kept kept;
-  kept.key = kMinusInfKey - 1u;  // every logit above -inf
+  kept.x = -FLT_MAX;  // every logit above -inf
   kept.last = 0x7FFFFFFF;
   bool all = true;               // as long as that is so, the weights alone tell
 
   // ---- top-k ------------------------------------------------------------------------------
-  const int from = warp * row.chunk, to = min(row.n, from + row.chunk);
+  const int from = warp * row.chunk;
   if (top_k > 0 && top_k < p.vocab) {
     unsigned beyond = 0u;  // in the last bin, where most tokens are: counted apart
-    for (int i = from + lane; i < to; i += 32 * kWide) {
+    for (int i = from + lane; i < from + row.chunk; i += 32 * kWide) {
       float v[kWide];
 #pragma unroll
-      for (int j = 0; j < kWide; ++j) v[j] = i + 32 * j < to ? x[i + 32 * j] : -INFINITY;
+      for (int j = 0; j < kWide; ++j) v[j] = x[i + 32 * j];
 #pragma unroll
       for (int j = 0; j < kWide; ++j) {
         const int b = row.bin(v[j]);
@@ -878,12 +956,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     if (found.bin >= 0 && live > (u64)top_k) {
       if (found.before + found.amount <= (u64)kList) {
         // all tokens up to the end of this bin: the first block of the cluster goes on alone
-        for (int i = from + lane; i - lane < to; i += 32 * kWide) {
+        for (int i = from + lane; i < from + row.chunk; i += 32 * kWide) {
           float v[kWide];
           bool chosen[kWide], any = false;
 #pragma unroll
           for (int j = 0; j < kWide; ++j) {
-            v[j] = i + 32 * j < to ? x[i + 32 * j] : -INFINITY;
+            v[j] = x[i + 32 * j];
             chosen[j] = v[j] != -INFINITY && row.upto_bin(v[j], found.bin);
             any |= chosen[j];
           }
@@ -916,25 +994,26 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   // ---- weights; top-p ---------------------------------------------------------------------
   const bool nucleus = top_p < 1.0f;
   u64 sum = 0ull;
-  for (int i = from + lane; i < to; i += 32 * kWide) {
+  for (int i = from + lane; i < from + row.chunk; i += 32 * kWide) {
     float v[kWide];
     u64 w[kWide];
+    int bin[kWide];
 #pragma unroll
     for (int j = 0; j < kWide; ++j) {
-      v[j] = i + 32 * j < to ? x[i + 32 * j] : -INFINITY;
-      w[j] = weigh(v[j]);
+      v[j] = x[i + 32 * j];
+      w[j] = weigh(v[j], bin[j]);
     }
     if (!all) {
 #pragma unroll
       for (int j = 0; j < kWide; ++j)
-        if (!kept.holds(descending_key(v[j]), row.base + i + 32 * j)) w[j] = 0ull;
+        if (!kept.holds(v[j], row.base + i + 32 * j)) w[j] = 0ull;
     }
 #pragma unroll
     for (int j = 0; j < kWide; ++j) sum += w[j];
     if (nucleus) {
 #pragma unroll
       for (int j = 0; j < kWide; ++j)
-        if (w[j]) add_mass<kBins>(sh.part[0], row.bin(v[j]), w[j]);
+        if (w[j]) add_mass<kBins>(sh.part[0], bin[j], w[j]);
     }
   }
   u64 total = 0ull;
@@ -945,33 +1024,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     if (found.bin >= 0 && need < total) {
       kept = select<true>(sh, cluster, row, weigh, kept, found.bin, need - found.before);
       all = false;
-      sum = 0ull;
-      for (int i = from + lane; i < to; i += 32 * kWide) {
-        bool wanted[kWide], any = false;
-        float v[kWide];
-#pragma unroll
-        for (int j = 0; j < kWide; ++j) {
-          v[j] = i + 32 * j < to ? x[i + 32 * j] : -INFINITY;
-          wanted[j] = kept.holds(descending_key(v[j]), row.base + i + 32 * j);
-          any |= wanted[j];
-        }
-        if (!any) continue;
-#pragma unroll
-        for (int j = 0; j < kWide; ++j) {
-          const u64 w = weigh(v[j]);
-          sum += wanted[j] ? w : 0ull;
-        }
-      }
+      sum = sum_kept(sh, row, weigh, kept);
     }
   }
   sum = warp_total(sum);
   if (lane == 0) sh.warp_sum[warp] = sum;
-  total = cluster_total(sh, cluster);
+  u64 before;
+  total = cluster_total(sh, cluster, before);
 
   // ---- draw -------------------------------------------------------------------------------
   const u64 target = draw_target(u, total);
-  u64 before = 0ull;
-  for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&sh.sum, r);
   cluster.sync();  // no block leaves while another reads its shared memory
   if (before <= target && target < before + sh.sum) {  // one block of the cluster
     // the warp whose tokens hold the target; its tokens, one per thread
@@ -986,7 +1048,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
       const int i = start + threadIdx.x;
       const float v = i < end ? x[i] : -INFINITY;
       u64 w = weigh(v);
-      if (!all && !kept.holds(descending_key(v), row.base + i)) w = 0ull;
+      if (!all && !kept.holds(v, row.base + i)) w = 0ull;
       u64 upto = inclusive_scan(w);
       __syncthreads();  // the sums before have been read
       if (lane == 31) sh.warp_sum[warp] = upto;
@@ -1027,7 +1089,7 @@ cudaError_t launch_sample(const void* logits, bool logits_f32, long long row_str
                                   (rows * blocks * 2 <= sm_count && vocab / blocks > 4096)))
     blocks *= 2;
   p.slice = (vocab + blocks - 1) / blocks;
-  const size_t bytes = sizeof(SampleShared) + (size_t)(p.slice + 3) * sizeof(float);
+  const size_t bytes = sizeof(SampleShared) + (size_t)((p.slice + kPad - 1) / kPad * kPad + 3) * sizeof(float);
   const void* kernel = logits_f32 ? (const void*)sample_kernel<float>
                                   : (const void*)sample_kernel<__nv_bfloat16>;
   static std::atomic<uint64_t> allowed[2];
