@@ -67,8 +67,8 @@ struct FewParams {
   unsigned long long inter_inverse;  // ceil(2^40 / inter)
   double* logits;           // [tokens, experts]
   uint32_t* act_max;        // [tokens * top_k]  E4M3 only: bit pattern of max |activation|
-  uint16_t* act_hi;         // [tokens * top_k, inter]  BF16 high parts; E4M3: FP32 bits 31..16
-  uint16_t* act_lo;         // BF16 low parts; E4M3: FP32 bits 15..0
+  uint16_t* act_hi;         // [tokens * top_k, inter]  BF16 high parts; E4M3: all bits, FP32
+  uint16_t* act_lo;         // BF16 low parts
   __nv_bfloat16* out;
   int64_t* ids_out;
   float* weights_out;
@@ -88,7 +88,7 @@ struct alignas(128) FewShared {
   signed char assign[kFewSlots][kFewMaxTokens];  // assignment of (slot, token), or -1
   uint32_t members[kFewSlots];          // tokens of a slot, one bit each
   float x_unscale[kFewMaxTokens];       // E4M3: 2^-s of the token rows
-  float a_scale[kFewSlots];             // E4M3: 2^s of the activation rows
+  float a_scale[kFewSlots], a_unscale[kFewSlots];  // E4M3: 2^s and 2^-s of the activation rows
   uint32_t x_max[kFewMaxTokens];
   int abort;
 };
@@ -725,20 +725,16 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
               up *= __ldg(s + p.inter) * sh.x_unscale[tok];
             }
             const float act = gate / (1.0f + expf(-gate)) * up * sh.weight[a];
-            uint16_t hi, lo;
             if constexpr (FP8) {
-              const uint32_t bits = __float_as_uint(act);
-              hi = (uint16_t)(bits >> 16);
-              lo = (uint16_t)bits;
-              atomicMax(&sh.act_max[a], bits & 0x7FFFFFFFu);
+              reinterpret_cast<float*>(p.act_hi)[(size_t)a * p.inter + col] = act;
+              atomicMax(&sh.act_max[a], __float_as_uint(act) & 0x7FFFFFFFu);
             } else {
               const __nv_bfloat16 high = __float2bfloat16_rn(act);
               const float rest = act - __bfloat162float(high);
-              hi = __bfloat16_as_ushort(high);
-              lo = __bfloat16_as_ushort(__float2bfloat16_rn(isfinite(rest) ? rest : 0.0f));
+              p.act_hi[(size_t)a * p.inter + col] = __bfloat16_as_ushort(high);
+              p.act_lo[(size_t)a * p.inter + col] =
+                  __bfloat16_as_ushort(__float2bfloat16_rn(isfinite(rest) ? rest : 0.0f));
             }
-            p.act_hi[(size_t)a * p.inter + col] = hi;
-            p.act_lo[(size_t)a * p.inter + col] = lo;
           }
         }
       }
@@ -752,12 +748,16 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
     if (threadIdx.x == 0) grid_arrive(p.sync + 1);
     ok = grid_wait(p.sync + 1, p.status, &sh.abort);
     if constexpr (FP8) {
-      if (threadIdx.x < p.tokens * p.top_k)
-        sh.a_scale[threadIdx.x] = row_scale(__ldcg(p.act_max + threadIdx.x));
+      if (threadIdx.x < p.tokens * p.top_k) {
+        const float scale = row_scale(__ldcg(p.act_max + threadIdx.x));
+        sh.a_scale[threadIdx.x] = scale;
+        sh.a_unscale[threadIdx.x] = 1.0f / scale;
+      }
       __syncthreads();
     }
 
     // ---- down ----------------------------------------------------------------------
+    const bool ragged = p.inter % (w.wide ? 2 * Work::kUnit : Work::kUnit) != 0;
 #pragma unroll 1
     for (int first = 0; ok && first < w.down_tiles; first += kFewMaxTiles) {
       float total[kFewMaxTiles][SUBS][4];
@@ -778,58 +778,68 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
         const int a = sh.assign[slot][g];
         // the tokens of this lane's two columns
         const unsigned members = sh.members[slot] >> (2 * t4);
-        uint32_t hi[SUBS][kWords], lo[SUBS][kWords];
         float row_scales[kFewMaxTiles][SUBS][2];
+        float u0 = 1.0f, u1 = 1.0f, scale = 1.0f;
         if constexpr (FP8) {
+          const float* sc =
+              p.down_scale + (size_t)sh.expert[slot] * p.hidden + w.row0 + first * w.down_height + g;
 #pragma unroll
           for (int r = 0; r < kFewMaxTiles; ++r)
 #pragma unroll
             for (int s = 0; s < SUBS; ++s) {
               const int i = (w.wide ? 0 : s * 16) + g, row = (first + r) * w.down_height + i;
-              const float* sc = p.down_scale + (size_t)sh.expert[slot] * p.hidden + w.row0 + row;
-              row_scales[r][s][0] = i < w.down_height && row < w.rows ? __ldg(sc) : 0.0f;
-              row_scales[r][s][1] = i + 8 < w.down_height && row + 8 < w.rows ? __ldg(sc + 8) : 0.0f;
+              const float* at = sc + r * w.down_height + (w.wide ? 0 : s * 16);
+              row_scales[r][s][0] = i < w.down_height && row < w.rows ? __ldg(at) : 0.0f;
+              row_scales[r][s][1] = i + 8 < w.down_height && row + 8 < w.rows ? __ldg(at + 8) : 0.0f;
             }
+          const int a0 = sh.assign[slot][2 * t4], a1 = sh.assign[slot][2 * t4 + 1];
+          if (a0 >= 0) u0 = sh.a_unscale[a0];
+          if (a1 >= 0) u1 = sh.a_unscale[a1];
+          if (a >= 0) scale = sh.a_scale[a];
         }
+        // The activations of the unit (wide: of both) for the lane's token.  With E4M3 weights a
+        // token that is not routed to this expert reads another row and its column is masked
+        // below: without the condition the eight loads of a lane go out together.
+        uint32_t hi[SUBS][kWords], lo[SUBS][kWords];
+        const bool whole = !(ragged && unit == w.units_i - 1);
+        const size_t act_row = (size_t)max(a, 0) * p.inter;
 #pragma unroll
         for (int s = 0; s < SUBS; ++s) {
           if (s && !w.wide) {  // both sub-tiles are of the same unit
 #pragma unroll
             for (int i = 0; i < kWords; ++i) {
               hi[s][i] = hi[0][i];
-              lo[s][i] = lo[0][i];
+              if (!FP8) lo[s][i] = lo[0][i];
             }
             break;
           }
           const int k = (w.wide ? 2 * unit + s : unit) * Work::kUnit + t4 * Work::kPiece;
-#pragma unroll
-          for (int i = 0; i < kWords / 4; ++i) {
-            const int at =
-                k + (FP8 ? (i / 2) * (Work::kUnit / 2) + (i % 2) * 8 : i * (Work::kUnit / 2));
-            uint4 q = make_uint4(0u, 0u, 0u, 0u), q2 = q;
-            if (a >= 0 && at < p.inter) {
-              q = __ldcg(reinterpret_cast<const uint4*>(p.act_hi + (size_t)a * p.inter + at));
-              q2 = __ldcg(reinterpret_cast<const uint4*>(p.act_lo + (size_t)a * p.inter + at));
-            }
-            hi[s][4 * i] = q.x; hi[s][4 * i + 1] = q.y; hi[s][4 * i + 2] = q.z; hi[s][4 * i + 3] = q.w;
-            lo[s][4 * i] = q2.x; lo[s][4 * i + 1] = q2.y; lo[s][4 * i + 2] = q2.z; lo[s][4 * i + 3] = q2.w;
-          }
           if constexpr (FP8) {
-            const float scale = a >= 0 ? sh.a_scale[a] : 1.0f;
+            const float4* from = reinterpret_cast<const float4*>(
+                reinterpret_cast<const float*>(p.act_hi) + act_row + k);
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-              const __half2 h = __floats2half2_rn(
-                  __uint_as_float(__byte_perm(lo[s][i], hi[s][i], 0x5410)) * scale,
-                  __uint_as_float(__byte_perm(lo[s][i], hi[s][i], 0x7632)) * scale);
-              hi[s][i] = *reinterpret_cast<const uint32_t*>(&h);
+            for (int i = 0; i < 8; ++i) {
+              const int at = (i / 4) * 16 + i % 4;  // in float4: the second half 64 elements on
+              float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (whole || k + 4 * at < p.inter) v = __ldcg(from + at);
+              const __half2 h0 = __floats2half2_rn(v.x * scale, v.y * scale);
+              const __half2 h1 = __floats2half2_rn(v.z * scale, v.w * scale);
+              hi[s][2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
+              hi[s][2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int at = k + i * (Work::kUnit / 2);
+              uint4 q = make_uint4(0u, 0u, 0u, 0u), q2 = q;
+              if (a >= 0 && at < p.inter) {
+                q = __ldcg(reinterpret_cast<const uint4*>(p.act_hi + (size_t)a * p.inter + at));
+                q2 = __ldcg(reinterpret_cast<const uint4*>(p.act_lo + (size_t)a * p.inter + at));
+              }
+              hi[s][4 * i] = q.x; hi[s][4 * i + 1] = q.y; hi[s][4 * i + 2] = q.z; hi[s][4 * i + 3] = q.w;
+              lo[s][4 * i] = q2.x; lo[s][4 * i + 1] = q2.y; lo[s][4 * i + 2] = q2.z; lo[s][4 * i + 3] = q2.w;
             }
           }
-        }
-        float u0 = 1.0f, u1 = 1.0f;
-        if constexpr (FP8) {
-          const int a0 = sh.assign[slot][2 * t4], a1 = sh.assign[slot][2 * t4 + 1];
-          if (a0 >= 0) u0 = 1.0f / sh.a_scale[a0];
-          if (a1 >= 0) u1 = 1.0f / sh.a_scale[a1];
         }
 #pragma unroll
         for (int r = 0; r < kFewMaxTiles; ++r) {
