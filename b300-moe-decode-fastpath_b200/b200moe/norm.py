@@ -84,31 +84,37 @@ def _launch(x, residual, weight, eps, rows: int, out, scale, residual_out) -> No
     count = rows * hidden
     x_at, w_at, out_at = x.data_ptr(), weight.data_ptr(), out.data_ptr()
     w_f32 = weight.dtype is torch.float32
-    w_end = w_at + hidden * (4 if w_f32 else 2)
     out_size = 2 if scale is None else 1
-    # (start, end, element size) of what is read row by row, and of what is written
-    read = [(x_at, x_at + 2 * count, 2)]
-    written = [(out_at, out_at + out_size * count, out_size)]
+    x_end, out_end = x_at + 2 * count, out_at + out_size * count
+    w_end = w_at + (4 if w_f32 else 2) * hidden
     r_at = kept_at = scale_at = None
     r_f32 = False
+    r_size, r_end, kept_end = 0, 0, 0
     if residual is not None:
         r_f32 = residual.dtype is torch.float32
-        size = 4 if r_f32 else 2
+        r_size = 4 if r_f32 else 2
         r_at, kept_at = residual.data_ptr(), residual_out.data_ptr()
-        read.append((r_at, r_at + size * count, size))
-        written.append((kept_at, kept_at + size * count, size))
+        r_end, kept_end = r_at + r_size * count, kept_at + r_size * count
+    # (start, end, element size; 0: never the same as an input) of every result
+    written = [(out_at, out_end, out_size)]
+    if residual is not None:
+        if out_at < kept_end and kept_at < out_end:
+            raise ValueError("the output tensors must not overlap")
+        written.append((kept_at, kept_end, r_size))
     if scale is not None:
         scale_at = scale.data_ptr()
-        written.append((scale_at, scale_at + 4 * rows, 0))
-    for i, (start, end, size) in enumerate(written):
-        for start2, end2, _ in written[i + 1:]:
-            if start < end2 and start2 < end:
-                raise ValueError("the output tensors must not overlap")
+        scale_end = scale_at + 4 * rows
+        if (scale_at < out_end and out_at < scale_end) or \
+                (residual is not None and scale_at < kept_end and kept_at < scale_end):
+            raise ValueError("the output tensors must not overlap")
+        written.append((scale_at, scale_end, 0))
+    for start, end, size in written:
         if start < w_end and w_at < end:
             raise ValueError("the output tensors must not overlap the weight")
-        for start2, end2, size2 in read:
-            if start < end2 and start2 < end and (start != start2 or size != size2):
-                raise ValueError("an output may only overlap an input by being that tensor")
+        if (start < x_end and x_at < end and (start != x_at or size != 2)) or \
+                (start < r_end and residual is not None and r_at < end
+                 and (start != r_at or size != r_size)):
+            raise ValueError("an output may only overlap an input by being that tensor")
     index = x.device.index
     args = (x_at, r_at, r_f32, w_at, w_f32, rows, hidden, eps, out_at if scale is None else None,
             None if scale is None else out_at, scale_at, kept_at,

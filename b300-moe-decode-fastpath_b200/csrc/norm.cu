@@ -92,6 +92,8 @@ add_rms_norm_kernel(const __nv_bfloat16* x, const R* residual, const W* __restri
   const bool live = row < rows;  // the last block's surplus rows only keep the barrier
   const size_t base = live ? (size_t)row * hidden : 0;
 
+  pdl_launch_dependents();
+  pdl_wait();
   // everything that a row needs is on its way before anything is waited for
   Raw8<__nv_bfloat16> rx[VECS];
   Raw8<R> rr[VECS];
@@ -177,11 +179,22 @@ cudaError_t launch_norm(const void* x, const void* residual, const void* weight,
   const dim3 block(threads, together);
   const dim3 grid((unsigned)((rows + together - 1) / together));
   auto run = [&](auto kernel) {
-    kernel<<<grid, block, 0, stream>>>(
-        static_cast<const __nv_bfloat16*>(x), static_cast<const R*>(residual),
-        static_cast<const W*>(weight), rows, hidden, eps, static_cast<__nv_bfloat16*>(out), codes,
-        scale, static_cast<R*>(residual_out));
-    return cudaGetLastError();
+    // With many rows the launch overlaps the end of the kernel in front, for which the kernel
+    // waits before it reads anything (4099 x 2880: 17.1 -> 16.6 us, 8192 x 4096 E4M3 37.2 -> 36.7
+    // us back to back; 64 x 7168 E4M3 3.6 -> 4.0 us).
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = block;
+    config.stream = stream;
+    config.attrs = &attr;
+    config.numAttrs = rows > kNormFewRows ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, static_cast<const __nv_bfloat16*>(x),
+                              static_cast<const R*>(residual), static_cast<const W*>(weight), rows,
+                              hidden, eps, static_cast<__nv_bfloat16*>(out), codes, scale,
+                              static_cast<R*>(residual_out));
   };
   if (per == 1) return run(add_rms_norm_kernel<R, W, FP8, 1>);
   if (per == 2) return run(add_rms_norm_kernel<R, W, FP8, 2>);
