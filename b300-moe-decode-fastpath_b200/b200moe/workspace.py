@@ -343,6 +343,10 @@ class B300MoEWorkspace:
                     backend,
                 )
                 self._signature = signature
+                if on_cuda:
+                    # the first call may come on another stream: it has to find the status area
+                    # cleared, which holds the grid-barrier counters of the one-kernel layer
+                    self._event.record(stream)
             else:
                 self._reuses += 1
             self._last_shape = (num_tokens, num_experts, top_k, hidden_size, intermediate_size)

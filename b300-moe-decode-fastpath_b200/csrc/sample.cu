@@ -8,22 +8,26 @@
 // A temperature that is not above zero takes the first token of the order.  NaN logits count as
 // -inf, tokens at -inf are never drawn; a row of nothing else gives -1.
 //
-// No sorting.  What is kept is a prefix of the order, so it is described by its last element: a
-// threshold on the logit and the index of the last token kept among those equal to it.  A
-// histogram over 2048 bins linear in m - x (for top-k of counts, for top-p of weights) finds the
-// bin in which the wanted sum is crossed; the few hundred tokens of that bin are collected in a
-// list and compared with one another.  Where top-k leaves few tokens altogether they are collected instead, and one block does the rest.  A bin with more than 1024 tokens
-// (equal logits, a range far from that of the weights) is taken apart by three histograms over
-// the digits (11, 11 and 10 bits) of the logit's ordered bit pattern.  A row is read from memory
-// once and stays in the shared memory of a cluster of up to eight blocks, which exchange
-// histograms, lists and sums as distributed shared memory.
+// No sorting of the row.  What is kept is a prefix of the order, so it is described by its last
+// element: a threshold on the logit and the index of the last token kept among those equal to it.
+// A histogram over 2048 bins linear in the logit (for top-k of counts, for top-p of weights) finds
+// the bin in which the wanted sum is crossed; the few hundred tokens of that bin are collected in
+// a list, narrowed down by a second histogram over 256 pieces of the bin and compared with one
+// another.  Where top-k leaves few tokens altogether they are collected instead, and one block
+// does the rest.  A bin with more than 1024 tokens (equal logits, a range far from that of the
+// weights) is taken apart by three histograms over the digits (11, 11 and 10 bits) of the logit's
+// ordered bit pattern.  A row is read from memory once and stays in the shared memory of a cluster
+// of up to eight blocks, which exchange histograms, lists and sums as distributed shared memory.
 //
-// What bounds it.  One to a few rows: the chain of load, four to five cluster barriers and two
-// passes over shared memory.  Many rows: the FP64 exponentials (12 instructions a token and
-// pass) and the histogram's atomics.  Shared-memory atomics of 64 bits are loops of
-// compare-and-swap (9,000 to 16,000 cycles for 16,384 tokens, 240,000 where they meet in four
-// bins), those of 32 bits are not (1,300 and 4,300), so a weight is added as three parts of 15
-// bits.
+// What bounds it.  Few rows: the chain of load, four to five cluster barriers (0.23 us each, a
+// remote read 0.37 us) and two passes over shared memory: 14.4 us for top-p over 32000 tokens,
+// 13.3 us for 17 rows of 32003 with top-k and top-p, 11.1 us for plain draws from 8 rows of
+// 129280.  Many rows: the FP64 exponentials, twelve operations a token and pass, the integer
+// work around them and the histogram's atomics: 64 rows of 129280 in 34.7 us plain, 75 us with
+// top-p 0.9, 37.6 us with top-k, 48.5 us mixed (5.0 us for the bytes alone).  Shared-memory atomics
+// of 64 bits are loops of compare-and-swap (9,000 to 16,000 cycles for 16,384 tokens, 240,000
+// where they meet in four bins), those of 32 bits are not (1,300 and 4,300), so a weight is added
+// as three parts of 15 bits.
 //
 // Exact sums.  With a large vocabulary the borders between tokens lie closer together than FP32
 // sums resolve, and sums in another order would move them.  The weights are therefore integers,
@@ -31,9 +35,9 @@
 // depend on the order in which threads add them, and an atomic of integers leaves no trace of
 // who came first.  The exponential behind them is computed in FP64 to about 2^-49: reduction to
 // 2^(k/128) * 2^r with a table of 128 powers (Tang's table-driven scheme) and the Taylor
-// polynomial of degree 4 on |r| <= 2^-8.  A thread weighs four tokens at a time, without
-// branches: one after the other, each waiting for twelve dependent FP64 operations, they took
-// 15 us for 16,160 tokens of a block.
+// polynomial of degree 4 on |r| <= 2^-8.  A thread weighs four tokens at a time and without
+// branches, so that their chains of dependent FP64 operations overlap (a pass over a block's
+// 16,160 tokens: 4.7 us against 6.4 us).
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -60,7 +64,9 @@ constexpr int kPad = kSampleThreads * kWide;
 constexpr int kPartBits = 15;
 constexpr int kGroups = 64;            // groups of 32 bins
 constexpr int kList = 1024;            // tokens of a list
-constexpr int kPairs = 256;            // up to so many are compared with one another, else sorted
+// Lists of up to so many tokens are compared pair by pair, longer ones sorted: two sorts of 64 to
+// 128 tokens take 4 us, two comparisons 1 us, but the work of a comparison grows with the square.
+constexpr int kPairs = 256;
 constexpr int kPieces = 256;           // of a bin
 
 struct SampleParams {
@@ -1084,9 +1090,13 @@ cudaError_t launch_sample(const void* logits, bool logits_f32, long long row_str
   p.min_p_v = min_p_v;
   p.ids = ids;
   p.logprobs = logprobs;
+  // Blocks of a row: as many as keep a block's tokens at 16384 or fewer, so that two blocks share
+  // an SM (64 rows of 129280 mixed: 48.5 us against 55.6 us with 32768); and while SMs are left
+  // and a block has more than 1536 tokens, more (one row of 32000, top-p: 14.4 us with eight
+  // against 22.4 us with two; of 8000: 13.1 us with eight against 14.2 us with two).
   int blocks = 1;
   while (blocks < kMaxCluster && ((vocab + blocks - 1) / blocks > 16384 ||
-                                  (rows * blocks * 2 <= sm_count && vocab / blocks > 4096)))
+                                  ((long long)rows * blocks * 2 <= sm_count && vocab / blocks > 1536)))
     blocks *= 2;
   p.slice = (vocab + blocks - 1) / blocks;
   const size_t bytes = sizeof(SampleShared) + (size_t)((p.slice + kPad - 1) / kPad * kPad + 3) * sizeof(float);

@@ -287,3 +287,23 @@ def test_streams_and_graphs(cuda_device) -> None:
         with torch.cuda.graph(graph):
             b300_moe_layer(held, r, gate_up, down, num_experts=16, top_k=4)
     assert torch.equal(b300_moe_layer(x, r, gate_up, down, **options), want_x)
+
+
+def test_a_workspace_reserved_on_a_busy_stream_is_used_on_another(cuda_device) -> None:
+    """The clearing of the workspace's status area is queued behind other work; the first call, on
+    another stream, waits for it."""
+
+    x, r, gate_up, down = _inputs(cuda_device, 2, 256, 128, 8)
+    want = b300_moe_layer(x, r, gate_up, down, num_experts=8, top_k=2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    junk = torch.full((1 << 20,), 255, dtype=torch.uint8, device=cuda_device)
+    del junk  # so that the workspace may get memory that is not zero
+    ws = B300MoEWorkspace(2, device=cuda_device)
+    torch.cuda._sleep(20_000_000)  # about 10 ms
+    ws.reserve(num_tokens=2, num_experts=8, top_k=2, hidden_size=256, intermediate_size=128,
+               device=cuda_device, dtype=torch.bfloat16, backend="b200_bf16", quant_mode="bf16")
+    with torch.cuda.stream(side):
+        got = b300_moe_layer(x, r, gate_up, down, num_experts=8, top_k=2, workspace=ws)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and ws.status() == 0
