@@ -138,7 +138,7 @@ struct ScratchLayout {
   size_t a_amax;     // uint32 [rows_cap]  bit pattern of max |activation| per row
   size_t few_logits; // b200moe_layer only: fp64 [kFewMaxTokens, experts],
   size_t few_amax;   //   uint32 [8 * kFewMaxTokens]  bit pattern of max |activation| per row,
-  size_t few_acts;   //   4 bytes [min(rows_cap, 8 * kFewMaxTokens), I]  activations
+  size_t few_acts;   //   4 bytes [min(rows_cap, 8 * kFewMaxTokens), I to whole 64]  activations
   size_t total;
 };
 
@@ -172,7 +172,7 @@ __host__ __device__ inline ScratchLayout scratch_layout(int rows_cap, int expert
                         kScratchAlign);
   l.few_acts = align_up(l.few_amax + 8 * kFewMaxTokens * sizeof(uint32_t), kScratchAlign);
   const int few_rows = rows_cap < 8 * kFewMaxTokens ? rows_cap : 8 * kFewMaxTokens;
-  l.total = align_up(l.few_acts + (size_t)few_rows * inter * 4, kScratchAlign);
+  l.total = align_up(l.few_acts + few_rows * align_up((size_t)inter, 64) * 4, kScratchAlign);
   return l;
 }
 

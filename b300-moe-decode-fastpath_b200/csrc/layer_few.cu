@@ -19,16 +19,21 @@
 //
 // The tile.  A warp multiplies 16 or 32 rows by 8 columns with mma.m16n8k16.  The column index
 // is the token, for gate/up and down alike, so the token operand needs no gathering: for gate+up
-// all tokens are multiplied and only those routed to the expert are kept; for down the other
-// tokens' columns are zero and are masked once more when a unit's tile is added (a weight of NaN
-// or infinity reaches only the tokens routed to it).  mma.sync and not tcgen05: 8 columns of
+// all tokens are multiplied and only those routed to the expert are kept; for down the columns
+// of the other tokens (zero, with E4M3 weights some other row) are masked when a unit's tile is
+// added: a weight of NaN or infinity reaches only the tokens routed to it.  mma.sync and not tcgen05: 8 columns of
 // useful work leave the tensor pipe idle either way, and operands that arrive in registers need
 // no descriptor, no tensor memory and no block-wide handshake per tile.
+//   Measured (weights from HBM, in a graph; copy rate 6.56 TB/s): H = 2048, I = 768, 128 experts,
+// top-8: 25.4 us for one token (floor 11.6: 7 us go by before the first weight, 3 us at the second
+// barrier), 98 to 106 us for eight (73.9; SMs end gate+up up to 9 us apart); H = 4096, I = 14336,
+// 8 experts, top-2: 118 us (107) and 422 us (412); E4M3 80 and 253 us (206) at the two shapes for
+// eight tokens, 106 us (68) for three with H = I = 2880, 32 experts, top-8, where 20 output rows a
+// block fill 32 rows of MMAs (without the MMAs 16 us less, without loading activations 9 us less).
 //
 // Loads.  Each lane copies with cp.async the very 16 bytes that it will use as fragments (rows
 // g and g+8, four lanes side by side in a row), into a ring of its warp in shared memory, and
-// reads them back itself: no barrier between producer and consumer, and up to 192 KB in flight
-// on an SM.  Any permutation of the reduction dimension is allowed as long as both operands
+// reads them back itself: no barrier between producer and consumer.  Any permutation of the reduction dimension is allowed as long as both operands
 // share it, which is why a lane's 16 consecutive bytes can serve as its part of the fragment.
 // The ring does not stop at the grid barrier: while a block waits for the activations, its
 // warps' first down tiles are already on their way.
@@ -53,7 +58,12 @@ namespace {
 constexpr int kFewWarps = 16;
 constexpr int kFewThreads = kFewWarps * 32;
 constexpr int kFewSlots = kFewMaxTokens * 8;  // experts in use, at most; also assignments
-constexpr int kFewMaxTiles = 2;               // down tiles that share one load of the activations
+// Stages of a warp's ring.  Two, 64 KB (32 rows a stage: 128 KB) of an SM in flight, cover the
+// latency of HBM; with a third the copies of all warps queue longer in front of the loads of
+// activations (BF16, 8 tokens, H = 4096, I = 14336, 8 experts: 422 us against 434 us with three or
+// four; H = 2048, I = 768, 128 experts: 97.6 against 98.8 us; but one token, H = I = 2880:
+// 84.5 against 79.5 us).
+constexpr int kFewStages = 2;
 
 struct FewParams {
   const __nv_bfloat16* x;
@@ -67,7 +77,8 @@ struct FewParams {
   unsigned long long inter_inverse;  // ceil(2^40 / inter)
   double* logits;           // [tokens, experts]
   uint32_t* act_max;        // [tokens * top_k]  E4M3 only: bit pattern of max |activation|
-  uint16_t* act_hi;         // [tokens * top_k, inter]  BF16 high parts; E4M3: all bits, FP32
+  uint16_t* act_hi;         // [tokens * top_k, inter]  BF16 high parts; E4M3: FP32, in the
+  int act_pitch;            //   order of act_place, `act_pitch` elements a row
   uint16_t* act_lo;         // BF16 low parts
   __nv_bfloat16* out;
   int64_t* ids_out;
@@ -162,6 +173,15 @@ __device__ __forceinline__ void multiply_piece(float (&c)[4], const uint4& top, 
     for (int i = 0; i < 2; ++i)
       mma_16x8x16<false>(c, t[2 * i], u[2 * i], t[2 * i + 1], u[2 * i + 1], b[2 * i], b[2 * i + 1]);
   }
+}
+
+// Where element `col` of an FP32 activation row lies.  The down projection's lane t of four takes
+// elements 16 t .. 16 t + 15 of each run of 64, four at a time: with the fours of the four lanes
+// side by side one load reads whole sectors, in plain order it reads half of each, and L2 delivers
+// three times the bytes of the weights (8 tokens, H = 4096, I = 14336, 8 experts: 284 -> 263 us;
+// H = 2048, I = 768, 128 experts: 99 -> 81 us).
+__device__ __forceinline__ int act_place(int col) {
+  return (col & ~63) | ((col & 12) << 2) | ((col >> 2) & 12) | (col & 3);
 }
 
 // Grid barrier in two halves: arrive (one thread, for the stores that come before it), then wait
@@ -312,8 +332,8 @@ __device__ __forceinline__ void router_logits(const FewParams& p, Shared& sh,
 }
 
 // Top-k of every token, one warp each, then the list of experts in use.  Every block does this
-// for itself from the logits.  The candidates are compared as FP32, which rounds the 64-bit logits monotonically; only
-// where two are equal as FP32 do the 64 bits decide, and then the lower id.
+// for itself from the logits.  The candidates are compared as FP32, which rounds the 64-bit logits
+// monotonically; only where two are equal as FP32 do the 64 bits decide, and then the lower id.
 template <typename Shared>
 __device__ __forceinline__ void choose_experts(const FewParams& p, Shared& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -406,7 +426,8 @@ __device__ __forceinline__ void softmax_weights(const FewParams& p, Shared& sh) 
 
 // What one block does, and the order in which a warp's ring is filled: first the gate/up tiles,
 // then the down tiles.  Both sides of the ring -- the copies and the products -- walk it.
-template <bool FP8, int SUBS>
+// TILES: down tiles that share one load of the activations.
+template <bool FP8, int SUBS, int TILES>
 struct FewWork {
   static constexpr int kUnit = FP8 ? 128 : 64;   // elements of a row in one stage (128 bytes)
   static constexpr int kPiece = FP8 ? 16 : 8;    // elements in 16 bytes
@@ -425,6 +446,8 @@ struct FewWork {
     rows = (int)((unsigned)p.hidden * (blockIdx.x + 1u) / gridDim.x) - row0;
     down_tiles = (rows + 16 * SUBS - 1) / (16 * SUBS);
     down_height = down_tiles ? (rows + down_tiles - 1) / down_tiles : 0;
+    // a block with few output rows fills the stage with a second unit of them (E4M3, 4 tokens,
+    // H = 2048, I = 2880: 75 us, with half the stage empty 86 us)
     wide = SUBS == 2 && down_height <= 16;
     const int unit = wide ? 2 * kUnit : kUnit;
     units_h = (p.hidden + kUnit - 1) / kUnit;
@@ -448,9 +471,9 @@ struct FewWork {
 };
 
 // Fills the ring: one stage per call, in order.
-template <bool FP8, int SUBS, int STAGES, typename Shared>
+template <bool FP8, int SUBS, int TILES, typename Shared>
 struct FewProducer {
-  using Work = FewWork<FP8, SUBS>;
+  using Work = FewWork<FP8, SUBS, TILES>;
   const FewParams& p;
   const Shared& sh;
   const Work& w;
@@ -468,7 +491,7 @@ struct FewProducer {
 
   __device__ FewProducer(const FewParams& p_, const Shared& sh_, const Work& w_, uint32_t ring,
                          int warp_, int lane_)
-      : p(p_), sh(sh_), w(w_), dst(ring), ring_end(ring + STAGES * Work::kStageBytes), warp(warp_),
+      : p(p_), sh(sh_), w(w_), dst(ring), ring_end(ring + kFewStages * Work::kStageBytes), warp(warp_),
         lane(lane_), unit(warp_) {
     up_bytes = (size_t)p.inter * p.hidden * Work::kElem;
     set_tail(p.hidden, w.units_h, 1);
@@ -518,7 +541,7 @@ struct FewProducer {
       if (++slot == w.slots) {
         slot = 0;
         unit = warp;
-        tile += kFewMaxTiles;
+        tile += TILES;
         done = tile >= w.down_tiles;
       }
     }
@@ -559,7 +582,7 @@ struct FewProducer {
         copy(dst + s * 2048 + 1024, a + stride8, live8 && m0, live8 && m1, p.down);
         a += w.wide ? (size_t)128 : 2 * stride8;
       }
-      if (++sub == kFewMaxTiles || tile + sub == w.down_tiles) {
+      if (++sub == TILES || tile + sub == w.down_tiles) {
         sub = 0;
         unit += kFewWarps;
         if (unit >= w.units_i) enter_down();
@@ -567,13 +590,13 @@ struct FewProducer {
     }
     cp_async_commit();  // an empty group when there is nothing left
     dst += Work::kStageBytes;
-    if (dst == ring_end) dst -= STAGES * Work::kStageBytes;
+    if (dst == ring_end) dst -= kFewStages * Work::kStageBytes;
   }
 };
 
-template <bool FP8, bool ROUTER_F32, int SUBS, int STAGES>
+template <bool FP8, bool ROUTER_F32, int SUBS, int TILES>
 __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewParams p) {
-  using Work = FewWork<FP8, SUBS>;
+  using Work = FewWork<FP8, SUBS, TILES>;
   using Shared = FewShared<SUBS>;
   constexpr int kWords = FP8 ? 16 : 8;  // 32-bit words of the token operand in one unit
   extern __shared__ __align__(128) uint8_t smem[];
@@ -650,11 +673,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
   if (ok) {
     choose_experts(p, sh);
     w.deal_pairs(p, sh.used);
-    uint32_t src = rings + warp * STAGES * Work::kStageBytes + lane * 16;
-    const uint32_t ring_end = src + STAGES * Work::kStageBytes;
-    FewProducer<FP8, SUBS, STAGES, Shared> producer(p, sh, w, src, warp, lane);
+    uint32_t src = rings + warp * kFewStages * Work::kStageBytes + lane * 16;
+    const uint32_t ring_end = src + kFewStages * Work::kStageBytes;
+    FewProducer<FP8, SUBS, TILES, Shared> producer(p, sh, w, src, warp, lane);
 #pragma unroll 1
-    for (int i = 0; i < STAGES; ++i) producer.next();
+    for (int i = 0; i < kFewStages; ++i) producer.next();
     softmax_weights(p, sh);
 
     // ---- gate + up -----------------------------------------------------------------
@@ -678,7 +701,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
                        (FP8 ? (i / 2) * Work::kUnit + (i % 2) * 16 : i * Work::kUnit));
           b[4 * i] = q.x; b[4 * i + 1] = q.y; b[4 * i + 2] = q.z; b[4 * i + 3] = q.w;
         }
-        cp_async_wait<STAGES - 1>();
+        cp_async_wait<kFewStages - 1>();
         uint4 a[SUBS][4];
 #pragma unroll
         for (int s = 0; s < SUBS; ++s)
@@ -686,7 +709,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
           for (int i = 0; i < 4; ++i) a[s][i] = lds128(src + s * 2048 + i * 512);
         producer.next();
         src += Work::kStageBytes;
-        if (src == ring_end) src -= STAGES * Work::kStageBytes;
+        if (src == ring_end) src -= kFewStages * Work::kStageBytes;
 #pragma unroll
         for (int s = 0; s < SUBS; ++s) {
           multiply_piece<FP8>(c[s], a[s][0], a[s][2], b);
@@ -726,7 +749,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
             }
             const float act = gate / (1.0f + expf(-gate)) * up * sh.weight[a];
             if constexpr (FP8) {
-              reinterpret_cast<float*>(p.act_hi)[(size_t)a * p.inter + col] = act;
+              reinterpret_cast<float*>(p.act_hi)[(size_t)a * p.act_pitch + act_place(col)] = act;
               atomicMax(&sh.act_max[a], __float_as_uint(act) & 0x7FFFFFFFu);
             } else {
               const __nv_bfloat16 high = __float2bfloat16_rn(act);
@@ -746,6 +769,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
     }
     __syncthreads();
     if (threadIdx.x == 0) grid_arrive(p.sync + 1);
+    // the scales of this block's output rows, experts one after another, where the token rows were
+    float* scales = reinterpret_cast<float*>(x_rows);
+    if constexpr (FP8)
+      for (int i = threadIdx.x; i < w.slots * w.rows; i += kFewThreads) {
+        const int sl = i / w.rows;
+        scales[i] = __ldg(p.down_scale + (size_t)sh.expert[sl] * p.hidden + w.row0 + (i - sl * w.rows));
+      }
     ok = grid_wait(p.sync + 1, p.status, &sh.abort);
     if constexpr (FP8) {
       if (threadIdx.x < p.tokens * p.top_k) {
@@ -759,10 +789,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
     // ---- down ----------------------------------------------------------------------
     const bool ragged = p.inter % (w.wide ? 2 * Work::kUnit : Work::kUnit) != 0;
 #pragma unroll 1
-    for (int first = 0; ok && first < w.down_tiles; first += kFewMaxTiles) {
-      float total[kFewMaxTiles][SUBS][4];
+    for (int first = 0; ok && first < w.down_tiles; first += TILES) {
+      float total[TILES][SUBS][4];
 #pragma unroll
-      for (int r = 0; r < kFewMaxTiles; ++r)
+      for (int r = 0; r < TILES; ++r)
 #pragma unroll
         for (int s = 0; s < SUBS; ++s)
 #pragma unroll
@@ -778,19 +808,18 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
         const int a = sh.assign[slot][g];
         // the tokens of this lane's two columns
         const unsigned members = sh.members[slot] >> (2 * t4);
-        float row_scales[kFewMaxTiles][SUBS][2];
+        float row_scales[TILES][SUBS][2];
         float u0 = 1.0f, u1 = 1.0f, scale = 1.0f;
         if constexpr (FP8) {
-          const float* sc =
-              p.down_scale + (size_t)sh.expert[slot] * p.hidden + w.row0 + first * w.down_height + g;
+          const float* sc = scales + slot * w.rows + first * w.down_height + g;
 #pragma unroll
-          for (int r = 0; r < kFewMaxTiles; ++r)
+          for (int r = 0; r < TILES; ++r)
 #pragma unroll
             for (int s = 0; s < SUBS; ++s) {
               const int i = (w.wide ? 0 : s * 16) + g, row = (first + r) * w.down_height + i;
               const float* at = sc + r * w.down_height + (w.wide ? 0 : s * 16);
-              row_scales[r][s][0] = i < w.down_height && row < w.rows ? __ldg(at) : 0.0f;
-              row_scales[r][s][1] = i + 8 < w.down_height && row + 8 < w.rows ? __ldg(at + 8) : 0.0f;
+              row_scales[r][s][0] = i < w.down_height && row < w.rows ? at[0] : 0.0f;
+              row_scales[r][s][1] = i + 8 < w.down_height && row + 8 < w.rows ? at[8] : 0.0f;
             }
           const int a0 = sh.assign[slot][2 * t4], a1 = sh.assign[slot][2 * t4 + 1];
           if (a0 >= 0) u0 = sh.a_unscale[a0];
@@ -802,7 +831,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
         // below: without the condition the eight loads of a lane go out together.
         uint32_t hi[SUBS][kWords], lo[SUBS][kWords];
         const bool whole = !(ragged && unit == w.units_i - 1);
-        const size_t act_row = (size_t)max(a, 0) * p.inter;
+        const size_t act_row = (size_t)max(a, 0) * p.act_pitch;
 #pragma unroll
         for (int s = 0; s < SUBS; ++s) {
           if (s && !w.wide) {  // both sub-tiles are of the same unit
@@ -813,15 +842,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
             }
             break;
           }
-          const int k = (w.wide ? 2 * unit + s : unit) * Work::kUnit + t4 * Work::kPiece;
+          const int start = (w.wide ? 2 * unit + s : unit) * Work::kUnit;
+          const int k = start + t4 * Work::kPiece;
           if constexpr (FP8) {
             const float4* from = reinterpret_cast<const float4*>(
-                reinterpret_cast<const float*>(p.act_hi) + act_row + k);
+                                     reinterpret_cast<const float*>(p.act_hi) + act_row + start) + t4;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int at = (i / 4) * 16 + i % 4;  // in float4: the second half 64 elements on
+            for (int i = 0; i < 8; ++i) {  // elements k + (0..15) and k + 64 + (0..15)
               float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              if (whole || k + 4 * at < p.inter) v = __ldcg(from + at);
+              if (whole || k + (i / 4) * 64 + i % 4 * 4 < p.inter) v = __ldcg(from + i * 4);
               const __half2 h0 = __floats2half2_rn(v.x * scale, v.y * scale);
               const __half2 h1 = __floats2half2_rn(v.z * scale, v.w * scale);
               hi[s][2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
@@ -842,9 +871,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
           }
         }
 #pragma unroll
-        for (int r = 0; r < kFewMaxTiles; ++r) {
+        for (int r = 0; r < TILES; ++r) {
           if (first + r >= w.down_tiles) break;
-          cp_async_wait<STAGES - 1>();
+          cp_async_wait<kFewStages - 1>();
           uint4 q[SUBS][4];
 #pragma unroll
           for (int s = 0; s < SUBS; ++s)
@@ -852,7 +881,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
             for (int i = 0; i < 4; ++i) q[s][i] = lds128(src + s * 2048 + i * 512);
           producer.next();
           src += Work::kStageBytes;
-          if (src == ring_end) src -= STAGES * Work::kStageBytes;
+          if (src == ring_end) src -= kFewStages * Work::kStageBytes;
 #pragma unroll
           for (int s = 0; s < SUBS; ++s) {
             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -884,7 +913,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
         for (int i = 0; i < 4; ++i) total[0][0][i] += total[0][SUBS - 1][i];
       }
 #pragma unroll
-      for (int r = 0; r < kFewMaxTiles; ++r) {
+      for (int r = 0; r < TILES; ++r) {
         if (first + r >= w.down_tiles) break;
         __syncthreads();  // the sums of the tile before are read
         if (2 * t4 < p.tokens) {
@@ -918,34 +947,36 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
   }
 }
 
-// Stage size and ring depth for a call whose token rows take `x_bytes` of shared memory: stages
-// of 32 rows (4 KB a warp) where two of them fit, because half as many loops, barriers and
-// token-operand loads go with a byte; of 16 rows where the token rows are longer.
+// Rows of a stage, tiles of a group, and the shared memory of a block for a call whose token rows
+// take `x_bytes` of it and whose blocks have up to `rows` output rows.
+//   Stages of 16 rows, groups of four tiles of the down projection.  BF16 with stages of 32 rows,
+// two tiles and a ring of three: 455 us instead of 422 us at 8 tokens, H = 4096, I = 14336,
+// 8 experts; 102.5 instead of 97.6 us at H = 2048, I = 768, 128 experts.  Two tiles of 16 rows:
+// the same where a block has no more, 431 instead of 418 us at H = 7168, I = 2048, 32 experts.
+//   E4M3, where a block has no more than 32 output rows (the token rows then leave the room on 148
+// SMs): stages of 32 rows, one tile.  That halves the loads and conversions of activations per byte of weights
+// (80 us against 90 us at H = 2048, I = 768, 128 experts; 106 against 124 us with 3 tokens,
+// H = I = 2880, 32 experts; 253 against 267 us at H = 4096, I = 14336, 8 experts); with more rows
+// a group of two such tiles does not fit in the registers (H = 7168, 8 tokens: 268 against 250 us).
 struct FewShape {
-  int subs, stages;
+  bool large;
   size_t bytes;
 };
-bool few_shape(size_t x_bytes, FewShape* shape) {
-  constexpr size_t kMost = kMostSharedMemory;
-  const FewShape options[4] = {{2, 3, 0}, {2, 2, 0}, {1, 3, 0}, {1, 2, 0}};
-  for (const FewShape& o : options) {
-    const size_t fixed = o.subs == 2 ? sizeof(FewShared<2>) : sizeof(FewShared<1>);
-    const size_t bytes = fixed + x_bytes + (size_t)o.stages * kFewWarps * o.subs * 2048;
-    if (bytes <= kMost) {
-      *shape = {o.subs, o.stages, bytes};
-      return true;
-    }
-  }
-  return false;
+FewShape few_shape(bool fp8, size_t x_bytes, int rows) {
+  constexpr size_t kRing = (size_t)kFewStages * kFewWarps * 2048;
+  const size_t large = sizeof(FewShared<2>) + x_bytes + 2 * kRing;
+  if (fp8 && rows <= 32 && large <= kMostSharedMemory) return {true, large};
+  return {false, sizeof(FewShared<1>) + x_bytes + kRing};
 }
+// the longest token rows fit
+static_assert(sizeof(FewShared<1>) + kFewMaxTokens * (B200MOE_LAYER_MAX_HIDDEN * 2 + 64) +
+                  kFewStages * kFewWarps * 2048 <= kMostSharedMemory, "shared memory");
 
 template <bool FP8, bool ROUTER_F32>
-const void* few_kernel(const FewShape& s) {
-  if (s.subs == 2)
-    return s.stages == 3 ? (const void*)layer_few_kernel<FP8, ROUTER_F32, 2, 3>
-                         : (const void*)layer_few_kernel<FP8, ROUTER_F32, 2, 2>;
-  return s.stages == 3 ? (const void*)layer_few_kernel<FP8, ROUTER_F32, 1, 3>
-                       : (const void*)layer_few_kernel<FP8, ROUTER_F32, 1, 2>;
+const void* few_kernel(bool large) {
+  if constexpr (FP8)
+    if (large) return (const void*)layer_few_kernel<true, ROUTER_F32, 2, 1>;
+  return (const void*)layer_few_kernel<FP8, ROUTER_F32, 1, 4>;
 }
 
 }  // namespace
@@ -979,20 +1010,20 @@ cudaError_t launch_layer_few(const void* x, const void* router, bool router_f32,
   p.act_max = act_max;
   p.act_hi = static_cast<uint16_t*>(acts);
   p.act_lo = p.act_hi + (size_t)tokens * top_k * inter;
+  p.act_pitch = (int)align_up((size_t)inter, 64);
   p.out = static_cast<__nv_bfloat16*>(out);
   p.ids_out = ids_out;
   p.weights_out = weights_out;
   p.sync = sync;
   p.status = status;
-  FewShape shape;
-  if (!few_shape(align_up((size_t)tokens * p.x_pitch, 128), &shape)) return cudaErrorInvalidValue;
-  const void* kernel = fp8 ? (router_f32 ? few_kernel<true, true>(shape)
-                                         : few_kernel<true, false>(shape))
-                           : (router_f32 ? few_kernel<false, true>(shape)
-                                         : few_kernel<false, false>(shape));
-  static std::atomic<uint64_t> allowed[2][2][2][2];
-  cudaError_t err = allow_shared_memory(
-      kernel, allowed[fp8][router_f32][shape.subs - 1][shape.stages - 2]);
+  const FewShape shape = few_shape(fp8, align_up((size_t)tokens * p.x_pitch, 128),
+                                   (hidden + sm_count - 1) / sm_count);
+  const void* kernel = fp8 ? (router_f32 ? few_kernel<true, true>(shape.large)
+                                         : few_kernel<true, false>(shape.large))
+                           : (router_f32 ? few_kernel<false, true>(shape.large)
+                                         : few_kernel<false, false>(shape.large));
+  static std::atomic<uint64_t> allowed[2][2][2];
+  cudaError_t err = allow_shared_memory(kernel, allowed[fp8][router_f32][shape.large]);
   if (err != cudaSuccess) return err;
   void* args[] = {&p};
   return cudaLaunchCooperativeKernel(kernel, dim3(sm_count), dim3(kFewThreads), args, shape.bytes,

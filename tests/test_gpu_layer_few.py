@@ -307,3 +307,30 @@ def test_a_workspace_reserved_on_a_busy_stream_is_used_on_another(cuda_device) -
         got = b300_moe_layer(x, r, gate_up, down, num_experts=8, top_k=2, workspace=ws)
     torch.cuda.synchronize()
     assert torch.equal(got, want) and ws.status() == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("tokens, hidden, inter, experts, top_k",
+                         [(8, 4736, 144, 8, 4), (5, 4752, 208, 16, 8), (8, 8192, 80, 8, 2),
+                          (3, 2368, 272, 4, 2), (4, 2384, 48, 32, 8), (2, 144, 16, 4, 1)])
+def test_output_rows_of_a_block(cuda_device, tokens, hidden, inter, experts, top_k, fp8) -> None:
+    """Both sides of 16, 32 and 48 output rows a block, and expert widths that end inside a run of
+    64 activations."""
+    x, r, gate_up, down = _inputs(cuda_device, tokens, hidden, inter, experts)
+    want_ids, want_weights = _route(x, r, top_k)
+    if fp8:
+        fw = quantize_expert_weights_fp8(gate_up, down)
+        out, ids, _ = b300_moe_layer_fp8(x, r, fw, num_experts=experts, top_k=top_k,
+                                         return_routing=True, check_status=True)
+
+        def matrix(q, scale):
+            return lambda e: q[e].view(torch.float8_e4m3fn).double() * scale[e].double()[:, None]
+
+        gate_up_of, down_of = (matrix(fw.gate_up_q, fw.gate_up_scale),
+                               matrix(fw.down_q, fw.down_scale))
+    else:
+        out, ids, _ = b300_moe_layer(x, r, gate_up, down, num_experts=experts, top_k=top_k,
+                                     return_routing=True, check_status=True)
+        gate_up_of, down_of = (lambda e: gate_up[e].double()), (lambda e: down[e].double())
+    assert torch.equal(ids, want_ids)
+    _check(out, *_formula(x, gate_up_of, down_of, ids, want_weights, fp8=fp8))
