@@ -20,16 +20,19 @@
 // The tile.  A warp multiplies 16 or 32 rows by 8 columns with mma.m16n8k16.  The column index
 // is the token, for gate/up and down alike, so the token operand needs no gathering: for gate+up
 // all tokens are multiplied and only those routed to the expert are kept; for down the columns
-// of the other tokens (zero, with E4M3 weights some other row) are masked when a unit's tile is
+// of the other tokens (zero, with E4M3 weights a copy) are masked when a unit's tile is
 // added: a weight of NaN or infinity reaches only the tokens routed to it.  mma.sync and not tcgen05: 8 columns of
 // useful work leave the tensor pipe idle either way, and operands that arrive in registers need
 // no descriptor, no tensor memory and no block-wide handshake per tile.
 //   Measured (weights from HBM, in a graph; copy rate 6.56 TB/s): H = 2048, I = 768, 128 experts,
 // top-8: 25.4 us for one token (floor 11.6: 7 us go by before the first weight, 3 us at the second
 // barrier), 98 to 106 us for eight (73.9; SMs end gate+up up to 9 us apart); H = 4096, I = 14336,
-// 8 experts, top-2: 118 us (107) and 422 us (412); E4M3 80 and 253 us (206) at the two shapes for
-// eight tokens, 106 us (68) for three with H = I = 2880, 32 experts, top-8, where 20 output rows a
-// block fill 32 rows of MMAs (without the MMAs 16 us less, without loading activations 9 us less).
+// 8 experts, top-2: 118 us (107) and 422 us (412); E4M3 74.5 us (37) and 246 us (206) at the two
+// shapes for eight tokens, 106 us (68) for three with H = I = 2880, 32 experts, top-8, where the
+// 20 output rows of a block fill 32 rows of MMAs (without the MMAs 16 us less, without loading
+// activations 9 us less).  The router's product, top-k and the regular path, in a graph: 45, 98,
+// 125 and 412 to 420 us; E4M3 227 us for eight tokens, 103 us for three, 34 us against 23 us for
+// one token at the first shape, 82 us against 73 us at the second.
 //
 // Loads.  Each lane copies with cp.async the very 16 bytes that it will use as fragments (rows
 // g and g+8, four lanes side by side in a row), into a ring of its warp in shared memory, and
@@ -96,7 +99,7 @@ struct alignas(128) FewShared {
   int chosen[kFewSlots];                // expert by assignment
   uint32_t act_max[kFewSlots];          // by assignment, of this block's activations
   uint32_t used[B200MOE_MAX_EXPERTS / 32];  // experts in use, one bit each
-  signed char assign[kFewSlots][kFewMaxTokens];  // assignment of (slot, token), or -1
+  signed char assign[kFewSlots][kFewMaxTokens];  // assignment of (slot, token), or below zero
   uint32_t members[kFewSlots];          // tokens of a slot, one bit each
   float x_unscale[kFewMaxTokens];       // E4M3: 2^-s of the token rows
   float a_scale[kFewSlots], a_unscale[kFewSlots];  // E4M3: 2^s and 2^-s of the activation rows
@@ -672,6 +675,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
 
   if (ok) {
     choose_experts(p, sh);
+    if constexpr (FP8) {  // a token that is not the expert's: ~(assignment of one that is)
+      const int slot = threadIdx.x / kFewMaxTokens, t = threadIdx.x % kFewMaxTokens;
+      const uint32_t members = sh.members[slot];
+      if (members && !(members >> t & 1u))
+        sh.assign[slot][t] = (signed char)~sh.assign[slot][__ffs(members) - 1];
+    }
     w.deal_pairs(p, sh.used);
     uint32_t src = rings + warp * kFewStages * Work::kStageBytes + lane * 16;
     const uint32_t ring_end = src + kFewStages * Work::kStageBytes;
@@ -827,11 +836,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
           if (a >= 0) scale = sh.a_scale[a];
         }
         // The activations of the unit (wide: of both) for the lane's token.  With E4M3 weights a
-        // token that is not routed to this expert reads another row and its column is masked
-        // below: without the condition the eight loads of a lane go out together.
+        // token that is not routed to this expert reads the row of one that is, and its column is
+        // masked below: without a condition the eight loads of a lane go out together (with one
+        // 145 us instead of 117 us at 3 tokens, H = I = 2880), and the bytes are in the same load
+        // anyway (with a row of another expert 255 us instead of 246 us at 8 tokens, H = 4096,
+        // I = 14336; 81 us instead of 74.5 us at H = 2048, I = 768, 128 experts).
         uint32_t hi[SUBS][kWords], lo[SUBS][kWords];
         const bool whole = !(ragged && unit == w.units_i - 1);
-        const size_t act_row = (size_t)max(a, 0) * p.act_pitch;
+        const size_t act_row = (size_t)(a < 0 ? ~a : a) * p.act_pitch;
 #pragma unroll
         for (int s = 0; s < SUBS; ++s) {
           if (s && !w.wide) {  // both sub-tiles are of the same unit
