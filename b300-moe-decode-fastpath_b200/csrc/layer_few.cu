@@ -20,10 +20,10 @@
 // The tile.  A warp multiplies 16 or 32 rows by 8 columns with mma.m16n8k16.  The column index
 // is the token, for gate/up and down alike, so the token operand needs no gathering: for gate+up
 // all tokens are multiplied and only those routed to the expert are kept; for down the columns
-// of the other tokens (zero, with E4M3 weights a copy) are masked when a unit's tile is
-// added: a weight of NaN or infinity reaches only the tokens routed to it.  mma.sync and not tcgen05: 8 columns of
-// useful work leave the tensor pipe idle either way, and operands that arrive in registers need
-// no descriptor, no tensor memory and no block-wide handshake per tile.
+// of the other tokens (zero, with E4M3 weights a copy) are masked when a unit's tile is added: a
+// weight of NaN or infinity reaches only the tokens routed to it.  mma.sync and not tcgen05: 8
+// columns of useful work leave the tensor pipe idle either way, and operands that arrive in
+// registers need no descriptor, no tensor memory and no block-wide handshake per tile.
 //   Measured (weights from HBM, in a graph; copy rate 6.56 TB/s): H = 2048, I = 768, 128 experts,
 // top-8: 25.4 us for one token (floor 11.6: 7 us go by before the first weight, 3 us at the second
 // barrier), 98 to 106 us for eight (73.9; SMs end gate+up up to 9 us apart); H = 4096, I = 14336,
@@ -36,8 +36,9 @@
 //
 // Loads.  Each lane copies with cp.async the very 16 bytes that it will use as fragments (rows
 // g and g+8, four lanes side by side in a row), into a ring of its warp in shared memory, and
-// reads them back itself: no barrier between producer and consumer.  Any permutation of the reduction dimension is allowed as long as both operands
-// share it, which is why a lane's 16 consecutive bytes can serve as its part of the fragment.
+// reads them back itself: no barrier between producer and consumer.  Any permutation of the
+// reduction dimension is allowed as long as both operands share it, which is why a lane's 16
+// consecutive bytes can serve as its part of the fragment.
 // The ring does not stop at the grid barrier: while a block waits for the activations, its
 // warps' first down tiles are already on their way.
 //
@@ -966,10 +967,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) layer_few_kernel(const FewPara
 // 8 experts; 102.5 instead of 97.6 us at H = 2048, I = 768, 128 experts.  Two tiles of 16 rows:
 // the same where a block has no more, 431 instead of 418 us at H = 7168, I = 2048, 32 experts.
 //   E4M3, where a block has no more than 32 output rows (the token rows then leave the room on 148
-// SMs): stages of 32 rows, one tile.  That halves the loads and conversions of activations per byte of weights
-// (80 us against 90 us at H = 2048, I = 768, 128 experts; 106 against 124 us with 3 tokens,
-// H = I = 2880, 32 experts; 253 against 267 us at H = 4096, I = 14336, 8 experts); with more rows
-// a group of two such tiles does not fit in the registers (H = 7168, 8 tokens: 268 against 250 us).
+// SMs): stages of 32 rows, one tile.  That halves the loads and conversions of activations per
+// byte of weights (80 us against 90 us at H = 2048, I = 768, 128 experts; 106 against 124 us with
+// 3 tokens, H = I = 2880, 32 experts; 253 against 267 us at H = 4096, I = 14336, 8 experts); with
+// more rows a group of two such tiles does not fit in the registers (H = 7168, 8 tokens: 268
+// against 250 us).
 struct FewShape {
   bool large;
   size_t bytes;
