@@ -63,7 +63,7 @@ def sample_tokens(
     gives -1.  ``return_logprobs=True`` also returns, in FP32, the logarithm of the probability
     with which the token was drawn (0 for the largest logit at ``temperature=0``, ``-inf`` with
     -1).  Rows may be further apart than V (a padded vocabulary: ``logits[:, :V]``); V is at most
-    262144.  ``out`` names where the ids go.
+    262144.  ``out`` names where the ids go; it must not overlap an input.
     """
 
     if not isinstance(logits, torch.Tensor) or not isinstance(uniforms, torch.Tensor):
@@ -112,6 +112,13 @@ def sample_tokens(
         if out.shape != (rows,) or out.dtype is not torch.int64 or out.device != device or \
                 not out.is_contiguous():
             raise ValueError(f"out must be a contiguous int64 [{rows}] tensor on the logits' device")
+        # a row's id is stored while other rows are still being read
+        start, end = out.data_ptr(), out.data_ptr() + 8 * rows
+        if any(at is not None and start < at + size and at < end for at, size in
+               ((logits.data_ptr(), ((rows - 1) * stride + vocab) * logits.element_size()),
+                (uniforms.data_ptr(), 4 * rows), (heat, 4 * rows), (k, 4 * rows), (p, 4 * rows),
+                (low, 4 * rows))):
+            raise ValueError("out must not overlap an input")
     if device.type != "cuda":
         raise ValueError("the native sampler requires CUDA tensors")
     ids = out if out is not None else torch.empty(rows, dtype=torch.int64, device=device)

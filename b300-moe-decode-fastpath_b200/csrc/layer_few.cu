@@ -181,9 +181,9 @@ __device__ __forceinline__ void multiply_piece(float (&c)[4], const uint4& top, 
 
 // Where element `col` of an FP32 activation row lies.  The down projection's lane t of four takes
 // elements 16 t .. 16 t + 15 of each run of 64, four at a time: with the fours of the four lanes
-// side by side one load reads whole sectors, in plain order it reads half of each, and L2 delivers
-// three times the bytes of the weights (8 tokens, H = 4096, I = 14336, 8 experts: 284 -> 263 us;
-// H = 2048, I = 768, 128 experts: 99 -> 81 us).
+// side by side one load reads whole sectors; in plain order it reads half of each, and every
+// sector is fetched twice (8 tokens, H = 4096, I = 14336, 8 experts: 284 -> 263 us; H = 2048,
+// I = 768, 128 experts: 99 -> 81 us).
 __device__ __forceinline__ int act_place(int col) {
   return (col & ~63) | ((col & 12) << 2) | ((col >> 2) & 12) | (col & 3);
 }
@@ -1030,6 +1030,11 @@ cudaError_t launch_layer_few(const void* x, const void* router, bool router_f32,
   p.weights_out = weights_out;
   p.sync = sync;
   p.status = status;
+  // the down scales of a block lie where its token rows were, which are longer on any GPU with
+  // more than 16 SMs
+  if (fp8 && (size_t)tokens * top_k * ((hidden + sm_count - 1) / sm_count) * sizeof(float) >
+                 (size_t)tokens * p.x_pitch)
+    return cudaErrorInvalidConfiguration;
   const FewShape shape = few_shape(fp8, align_up((size_t)tokens * p.x_pitch, 128),
                                    (hidden + sm_count - 1) / sm_count);
   const void* kernel = fp8 ? (router_f32 ? few_kernel<true, true>(shape.large)

@@ -72,3 +72,22 @@ def test_c_entry_checks_its_arguments() -> None:
     assert call(rows=0) == call(vocab=0) == call(stride=15) == -2
     assert call(rows=1048577) == call(vocab=262145, stride=262145) == -8
     assert call(logits=ctypes.c_void_p(4098)) == call(logits=ctypes.c_void_p(4097), f32=0) == -3
+
+
+@pytest.mark.parametrize("shared", ["logits", "uniforms", "temperature", "top_k", "top_p", "min_p"])
+def test_out_may_not_overlap_an_input(shared) -> None:
+    rows, vocab = 4, 16
+    held = torch.zeros(rows * vocab)
+    ids = held.view(torch.int64)[:rows]
+    inputs = {"logits": torch.zeros(rows, vocab), "uniforms": torch.zeros(rows)}
+    part = held.view(rows, vocab) if shared == "logits" else held[2 * rows - 1:3 * rows - 1]
+    inputs[shared] = part.view(torch.int32) if shared == "top_k" else part
+    with pytest.raises(ValueError, match="must not overlap an input"):
+        sample_tokens(inputs.pop("logits"), inputs.pop("uniforms"), out=ids, **inputs)
+
+
+def test_out_next_to_the_inputs_is_taken() -> None:
+    held = torch.zeros(4 + 8 + 4 + 64)
+    with pytest.raises(ValueError, match="requires CUDA"):  # all other checks have passed
+        sample_tokens(held[16:].view(4, 16), held[:4], temperature=held[12:16],
+                      out=held[4:12].view(torch.int64))
