@@ -25,7 +25,7 @@
 // columns of useful work leave the tensor pipe idle either way, and operands that arrive in
 // registers need no descriptor, no tensor memory and no block-wide handshake per tile.
 //   Measured (weights from HBM, in a graph; copy rate 6.56 TB/s): H = 2048, I = 768, 128 experts,
-// top-8: 25.4 us for one token (floor 11.6: 7 us go by before the first weight, 3 us at the second
+// top-8: 25.3 us for one token (floor 11.6: 7 us go by before the first weight, 3 us at the second
 // barrier), 98 to 106 us for eight (73.9; SMs end gate+up up to 9 us apart); H = 4096, I = 14336,
 // 8 experts, top-2: 118 us (107) and 422 us (412); E4M3 74.5 us (37) and 246 us (206) at the two
 // shapes for eight tokens, 106 us (68) for three with H = I = 2880, 32 experts, top-8, where the
@@ -357,18 +357,17 @@ __device__ __forceinline__ void choose_experts(const FewParams& p, Shared& sh) {
 #pragma unroll
       for (int i = 1; i < 8; ++i) best = max(best, key[i]);
       best = __reduce_max_sync(0xffffffffu, best);
-      int held = 0, at = 0;  // how many of this lane's keys are the best one, and the last of them
+      // how many keys are the best one (upper half), and the sum of their ids: of one, its id
+      unsigned id = 0u;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (key[i] == best) {
-          ++held;
-          at = i;
-        }
-      const unsigned holders = __ballot_sync(0xffffffffu, held != 0);
-      unsigned id;
-      if ((holders & (holders - 1u)) == 0u && !__any_sync(0xffffffffu, held > 1)) {
-        id = __shfl_sync(0xffffffffu, (unsigned)(lane + 32 * at), __ffs(holders) - 1);
+        if (key[i] == best) id += 0x10000u + (unsigned)(lane + 32 * i);
+      const bool held = id != 0u;
+      id = __reduce_add_sync(0xffffffffu, id);
+      if (id >> 16 == 1u) {
+        id &= 0xffffu;
       } else {
+        int at = 0;
         unsigned long long most = 0ull;  // among the equal ones, by all 64 bits
 #pragma unroll
         for (int i = 0; i < 8; ++i)
