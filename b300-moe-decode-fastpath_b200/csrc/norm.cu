@@ -5,7 +5,8 @@
 // is what is normalised: r' is a rounded copy of it.  No counterpart in the reference.
 //
 // A row is read once and stays in registers between the sum of its squares, the largest |y|
-// and the stores, so the kernel moves exactly the bytes of its operands: x, r, r', y.  Many rows
+// and the stores (of the longest rows up to 28 bytes a thread do not), so the kernel moves the
+// bytes of its operands: x, r, r', y.  Many rows
 // are bound by HBM: 8192 x 4096 in 41.4 us (6.48 TB/s, 0.99 of the measured copy rate), with E4M3
 // result 36.9 us (0.97); 4099 x 2880 E4M3 in 16.0 us (0.79: two waves of short rows).  One row
 // is bound by the latency of one load, one barrier and one store: 2.0 us for 4096 columns.
@@ -107,12 +108,19 @@ __device__ __forceinline__ uint32_t quotient_codes(const float (&y)[4], float sc
   return lo == hi ? lo : divided_codes(y[0], y[1], y[2], y[3], scale);
 }
 
-template <typename R, typename W, bool FP8, int VECS>
-__global__ void __launch_bounds__(1024)
+// THREADS: most threads of a block, which limits the registers of a thread to 65536 / THREADS
+template <typename R, typename W, bool FP8, int VECS, int THREADS = 1024>
+__global__ void __launch_bounds__(THREADS)
 add_rms_norm_kernel(const __nv_bfloat16* x, const R* residual, const W* __restrict__ weight,
                     long long rows, int hidden, float eps, __nv_bfloat16* out, uint8_t* codes,
                     float* scale_out, R* residual_out) {
   __shared__ float2 slots[32];
+  // Four vectors of a thread with a residual and an FP32 operand do not fit 64 registers when the
+  // weight waits in them as well: it is loaded vector by vector (FP32 residual and weight,
+  // 2048 x 32768: 139.6 us against 191 us with what was spilled; E4M3 with BF16 residual and FP32
+  // weight, 4096 x 7168: 36.0 against 38.2 us).
+  constexpr bool kLateWeight = VECS == 4 && THREADS == 1024 && !std::is_same<R, NormNone>::value &&
+                               (sizeof(R) == 4 || sizeof(W) == 4);
   const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
   const bool live = row < rows;  // the last block's surplus rows only keep the barrier
   const size_t base = live ? (size_t)row * hidden : 0;
@@ -129,7 +137,7 @@ add_rms_norm_kernel(const __nv_bfloat16* x, const R* residual, const W* __restri
     if (live && c < hidden) {
       rx[i].load(x + base + c);
       if constexpr (!std::is_same<R, NormNone>::value) rr[i].load(residual + base + c);
-      rw[i].load(weight + c);
+      if (!kLateWeight) rw[i].load(weight + c);
     }
   }
   // y = factor * t with t = s w and one factor per row, so that the largest |y| is known as soon
@@ -140,6 +148,7 @@ add_rms_norm_kernel(const __nv_bfloat16* x, const R* residual, const W* __restri
   for (int i = 0; i < VECS; ++i) {
     const int c = (threadIdx.x + i * blockDim.x) * 8;
     if (!(live && c < hidden)) continue;
+    if (kLateWeight) rw[i].load(weight + c);
     float s[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -221,6 +230,11 @@ cudaError_t launch_norm(const void* x, const void* residual, const void* weight,
   };
   if (per == 1) return run(add_rms_norm_kernel<R, W, FP8, 1>);
   if (per == 2) return run(add_rms_norm_kernel<R, W, FP8, 2>);
+  // Four vectors with an FP32 residual: blocks of up to 512 threads (H <= 16384) may have 73 to
+  // 102 registers a thread, with everything on its way at once (4096 x 7168, FP32 weight: 53.4 us
+  // against 57.5 us with the weight loaded late and 74.4 us with spills).
+  if constexpr (sizeof(R) == 4)
+    if (threads <= 512) return run(add_rms_norm_kernel<R, W, FP8, 4, 512>);
   return run(add_rms_norm_kernel<R, W, FP8, 4>);
 }
 
