@@ -108,10 +108,13 @@ __device__ __forceinline__ uint32_t quotient_codes(const float (&y)[4], float sc
   return lo == hi ? lo : divided_codes(y[0], y[1], y[2], y[3], scale);
 }
 
-// THREADS: most threads of a block, which limits the registers of a thread to 65536 / THREADS
+// THREADS: most threads of a block, which limits the registers of a thread to 65536 / THREADS.
+// No operand is __restrict__: that would promise that it is read-only from the kernel's start, and a
+// dependent launch starts while the kernel in front may still be storing it (a weight too: an
+// earlier norm's row, a copy of new parameters).
 template <typename R, typename W, bool FP8, int VECS, int THREADS = 1024>
 __global__ void __launch_bounds__(THREADS)
-add_rms_norm_kernel(const __nv_bfloat16* x, const R* residual, const W* __restrict__ weight,
+add_rms_norm_kernel(const __nv_bfloat16* x, const R* residual, const W* weight,
                     long long rows, int hidden, float eps, __nv_bfloat16* out, uint8_t* codes,
                     float* scale_out, R* residual_out) {
   __shared__ float2 slots[32];

@@ -1,4 +1,4 @@
-"""The residual norm's form for many rows.
+"""The residual norm's form for many rows, and launches that follow one another.
 
 Tolerances as in test_gpu_norm.py.
 """
@@ -32,3 +32,35 @@ def test_many_rows(cuda_device, rows, hidden, residual, weight) -> None:
     if r is not None:
         _check_residual(kept, s, r)
         assert torch.equal(kept8, kept)
+
+
+@pytest.mark.parametrize("hidden", [1024, 4096, 7168])
+def test_a_chain_of_norms_over_the_same_rows(cuda_device, hidden) -> None:
+    """Each launch may begin before the one in front has ended and reads what that one stores: the
+    rows, the residual and, in the third norm of a turn, the weight."""
+
+    x, r, w = _inputs(cuda_device, 1500, hidden, torch.float32, torch.bfloat16)
+
+    def turn(x, r, wait):
+        _, r = add_rms_norm(x, r, w, out=x, residual_out=r)
+        wait()
+        one, _ = add_rms_norm(x[:400], None, w)
+        wait()
+        row = one[7]                                  # a weight that the kernel in front stored
+        y, r = add_rms_norm(x, r, row, residual_out=r)
+        wait()
+        codes, scale, r = add_rms_norm_fp8(y, r, w, residual_out=r)
+        wait()
+        return y, r, codes, scale
+
+    def run(wait):
+        a, b, seen = x.clone(), r.clone(), []
+        for _ in range(6):
+            a, b, codes, scale = turn(a, b, wait)
+            seen += [codes, scale]
+        torch.cuda.synchronize()
+        return [a, b, *seen]
+
+    want = run(torch.cuda.synchronize)
+    for _ in range(5):
+        assert all(torch.equal(g, t) for g, t in zip(run(lambda: None), want))
