@@ -95,6 +95,9 @@ def _launch(x, residual, weight, eps, rows: int, out, scale, residual_out) -> No
         r_size = 4 if r_f32 else 2
         r_at, kept_at = residual.data_ptr(), residual_out.data_ptr()
         r_end, kept_end = r_at + r_size * count, kept_at + r_size * count
+    elif scale is None and out_at == x_at:
+        raise ValueError("without a residual, out must not be hidden_states: they are returned as "
+                         "the new residual")
     # (start, end, element size; 0: never the same as an input) of every result
     written = [(out_at, out_end, out_size)]
     if residual is not None:
@@ -161,7 +164,8 @@ def add_rms_norm(
 
     ``out`` and ``residual_out`` name where the results go instead of fresh tensors.  Each may
     be an input of its own dtype (``residual_out=residual`` updates the stream in place); no
-    other overlap is allowed.
+    other overlap is allowed, nor is ``out=hidden_states`` without a residual, since those are
+    then the new residual.
     """
 
     rows = _check(hidden_states, residual, weight, eps, 8)
