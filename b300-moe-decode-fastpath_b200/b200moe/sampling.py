@@ -55,7 +55,8 @@ def sample_tokens(
     Each setting is a number for all rows or a [T] tensor on the logits' device (FP32;
     ``top_k`` int32).  Off: ``top_k=0``, ``top_p=1``, ``min_p=0``.  ``temperature=0`` takes the
     largest logit.  Tensor values are not checked: a temperature that is not above 0 takes the
-    largest logit, ``top_k <= 0`` is off, ``top_p >= 1`` or NaN is off and ``top_p <= 0`` keeps
+    largest logit and an infinite one weighs all finite logits alike (beside an infinite logit
+    they weigh nothing), ``top_k <= 0`` is off, ``top_p >= 1`` or NaN is off and ``top_p <= 0`` keeps
     one token, ``min_p`` not above 0 is off and above 1 counts as 1; a uniform of 1 or more draws
     the last kept token.  Numbers are held in FP32.
 

@@ -931,8 +931,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
 
   Weigher weigh;
   weigh.set(sh.power, best, temperature, min_p);
-  // 2047 linear bins over the range of logits whose weight is not zero, one for the rest
-  row.scale = fminf((float)(2047.0 / 32.3) / temperature, 3.0e38f);
+  // 2047 linear bins over the range of logits whose weight is not zero, one for the rest.  Above
+  // zero also at an infinite temperature: logits that lie infinitely far apart (FP32's range, or
+  // one of them infinite) then fall into the last bin, where zero would make their bin NaN.
+  row.scale = fminf(fmaxf((float)(2047.0 / 32.3) / temperature, FLT_MIN), 3.0e38f);
 
   Kept kept;
   kept.x = -FLT_MAX;  // every logit above -inf

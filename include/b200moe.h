@@ -526,7 +526,8 @@ int b200moe_layer(const B200MoeArgs* args, const void* router_weight, int router
  *   temperature, top_k, top_p, min_p   [rows] on the device, or NULL: the value behind it for
  *                 every row.  Not above 0 / NaN: temperature takes the first of the order
  *                 (log-probability 0), top_k is off, top_p keeps one token (NaN: off), min_p is
- *                 off.  top_p >= 1 is off; min_p above 1 counts as 1.
+ *                 off.  top_p >= 1 is off; min_p above 1 counts as 1.  An infinite temperature
+ *                 weighs all finite logits alike, and beside an infinite logit with nothing.
  *   ids_out       [rows] int64 out
  *   logprobs_out  [rows] fp32 out or NULL: log of the probability that the token was drawn with
  */
