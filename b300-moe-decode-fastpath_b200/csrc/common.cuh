@@ -136,7 +136,9 @@ struct ScratchLayout {
   size_t x_scale;    // fp32 [rows_cap]
   size_t a_scale;    // fp32 [rows_cap]
   size_t a_amax;     // uint32 [rows_cap]  bit pattern of max |activation| per row
-  size_t few_logits; // b200moe_layer only: fp64 [kFewMaxTokens, experts],
+  // b200moe_layer only, over act_lo and what follows it, which hold nothing from one call to the
+  // next (the status area and the schedule in front are not touched):
+  size_t few_logits; //   fp64 [kFewMaxTokens, experts],
   size_t few_amax;   //   uint32 [8 * kFewMaxTokens]  bit pattern of max |activation| per row,
   size_t few_acts;   //   4 bytes [min(rows_cap, 8 * kFewMaxTokens), I to whole 64]  activations
   size_t total;
@@ -167,12 +169,14 @@ __host__ __device__ inline ScratchLayout scratch_layout(int rows_cap, int expert
   l.x_scale = align_up(l.q_planes + (size_t)kFp8Planes * rows_cap * widest, kScratchAlign);
   l.a_scale = align_up(l.x_scale + (size_t)rows_cap * sizeof(float), kScratchAlign);
   l.a_amax = align_up(l.a_scale + (size_t)rows_cap * sizeof(float), kScratchAlign);
-  l.few_logits = align_up(l.a_amax + (size_t)rows_cap * sizeof(uint32_t), kScratchAlign);
+  const size_t forward_end = l.a_amax + (size_t)rows_cap * sizeof(uint32_t);
+  l.few_logits = l.act_lo;
   l.few_amax = align_up(l.few_logits + (size_t)kFewMaxTokens * experts * sizeof(double),
                         kScratchAlign);
   l.few_acts = align_up(l.few_amax + 8 * kFewMaxTokens * sizeof(uint32_t), kScratchAlign);
   const int few_rows = rows_cap < 8 * kFewMaxTokens ? rows_cap : 8 * kFewMaxTokens;
-  l.total = align_up(l.few_acts + few_rows * align_up((size_t)inter, 64) * 4, kScratchAlign);
+  const size_t few_end = l.few_acts + few_rows * align_up((size_t)inter, 64) * 4;
+  l.total = align_up(few_end > forward_end ? few_end : forward_end, kScratchAlign);
   return l;
 }
 

@@ -504,7 +504,8 @@ int b200moe_router_topk(const void* logits, int logits_are_f32, int num_tokens, 
  *   weights_out   [T,K] fp32 out or NULL: the softmax weights, which are used unrounded
  * The first 256 bytes of scratch must be zero before the first call on it (they hold the
  * grid-barrier counters, which every call leaves at zero, and the status word).  A cooperative
- * launch of one block per SM; one scratch serves one call at a time.
+ * launch of one block per SM; one scratch serves one call at a time (stages of a forward on the
+ * same scratch included: what they leave there for one another is overwritten).
  */
 #define B200MOE_LAYER_MAX_TOKENS 8
 #define B200MOE_LAYER_MAX_HIDDEN 8192
