@@ -189,7 +189,9 @@ __device__ __forceinline__ int act_place(int col) {
 }
 
 // Grid barrier in two halves: arrive (one thread, for the stores that come before it), then wait
-// (the block; bounded, after that it goes on to its end without further work).
+// (the block; bounded, after that it goes on to its end without further work).  The counters are
+// compared as signed numbers: with one that starts below zero (a scratch that was not cleared)
+// no block passes, all give up, and the last one leaves the counters at zero for the next call.
 __device__ __forceinline__ void grid_arrive(unsigned int* counter) {
   asm volatile("fence.acq_rel.gpu;" ::: "memory");
   asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
@@ -201,7 +203,7 @@ __device__ __forceinline__ bool grid_wait(unsigned int* counter, uint32_t* statu
     while (true) {
       unsigned int seen;
       asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
-      if (seen >= gridDim.x) break;
+      if ((int)seen >= (int)gridDim.x) break;
       if ((++spins & 255u) == 0u && global_timer_ns() - t0 > 5ull * kPipeWaitLimitNs) {
         atomicOr(status, B200MOE_STATUS_PIPE_TIMEOUT);
         *abort = 1;
