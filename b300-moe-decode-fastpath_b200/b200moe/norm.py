@@ -158,7 +158,10 @@ def add_rms_norm(
 
     ``hidden_states`` [..., H] BF16, ``residual`` of the same shape in BF16 or FP32, ``weight``
     [H] in BF16 or FP32; contiguous, on one CUDA device, H a multiple of 8 and at most 32768.
-    The sum is normalised in FP32, before the rounding that stores it.  Without a residual
+    The sum is normalised in FP32, before the rounding that stores it; a row's result depends on
+    that row alone.  Squares and products with the weight are FP32 too: a row whose mean square
+    or products leave its range (elements beyond about 1e18) has no finite or meaningful result,
+    as in any FP32 norm.  Without a residual
     (``None``, the first norm of a model) ``hidden_states`` itself is normalised and returned
     as the new residual.
 

@@ -9,7 +9,7 @@
 // bytes of its operands: x, r, r', y.  Many rows
 // are bound by HBM: 8192 x 4096 in 41.4 us (6.48 TB/s, 0.99 of the measured copy rate), with E4M3
 // result 36.9 us (0.97); 4099 x 2880 E4M3 in 16.0 us (0.79: two waves of short rows).  One row
-// is bound by the latency of one load, one barrier and one store: 2.0 us for 4096 columns.
+// is bound by the latency of one load, one barrier and one store: 1.7 us for 4096 columns.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -23,11 +23,13 @@ namespace {
 constexpr float kNormE4m3Max = 448.0f;
 constexpr float kNormBracket = 1.0f / (1 << 21);
 constexpr float kNormLeastScale = 1.17549435e-38f;  // 2^-126, the smallest normal number
-// Up to two blocks per SM a row gets as many threads as it has vectors (64 rows of 7168: 3.6 us
-// against 4.8 us with 256 threads); with more rows 256 threads and several vectors each keep
-// more rows of an SM apart in time (4099 x 2880 E4M3: 16.0 us against 18.2 us; 8192 x 4096 E4M3:
-// 36.9 us against 44.2 us with 512).
-constexpr int kNormFewRows = 296;
+// Threads of a row: one for each vector up to 256, then two or four vectors each, whatever the
+// number of rows, so that a row's result depends on that row alone.  More threads keep fewer rows
+// of an SM apart in time (512: 8192 x 4096 E4M3 47.3 us against 38.3 us, 4099 x 2880 19.2 against
+// 16.6 us, though 4096 x 7168 with FP32 operands 52.6 against 55.1 us), and bring nothing where
+// rows are few (one for each vector up to 1024: 296 x 7168 4.2 us against 3.5 us, 1 x 16384 4.0
+// against 3.4 us, 64 x 2880 E4M3 2.5 against 2.65 us).
+constexpr int kNormThreads = 256;
 
 // eight consecutive elements, as they lie in memory; 16-byte accesses
 template <typename T>
@@ -206,17 +208,16 @@ cudaError_t launch_norm(const void* x, const void* residual, const void* weight,
                         void* residual_out, cudaStream_t stream) {
   const int vecs = hidden / 8;
   int per = 1;  // vectors of a thread
-  const int most = rows <= kNormFewRows ? 1024 : 256;
-  while (per < 4 && (vecs + per - 1) / per > most) per *= 2;
+  while (per < 4 && (vecs + per - 1) / per > kNormThreads) per *= 2;
   int threads = ((vecs + per - 1) / per + 31) / 32 * 32;
   int together = 1;  // rows of a block
   while (threads * together * 2 <= 256 && together < rows) together *= 2;
   const dim3 block(threads, together);
   const dim3 grid((unsigned)((rows + together - 1) / together));
   auto run = [&](auto kernel) {
-    // With many rows the launch overlaps the end of the kernel in front, for which the kernel
-    // waits before it reads anything (4099 x 2880: 17.1 -> 16.6 us, 8192 x 4096 E4M3 37.2 -> 36.7
-    // us back to back; 64 x 7168 E4M3 3.6 -> 4.0 us).
+    // The launch overlaps the end of the kernel in front, for which the kernel waits before it
+    // reads anything (1 x 4096: 2.05 -> 1.7 us, 4099 x 2880 16.4 -> 15.8 us, 8192 x 4096 E4M3 38.9
+    // -> 38.3 us back to back; 296 x 4096 2.9 -> 3.1 us).
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
@@ -225,7 +226,7 @@ cudaError_t launch_norm(const void* x, const void* residual, const void* weight,
     config.blockDim = block;
     config.stream = stream;
     config.attrs = &attr;
-    config.numAttrs = rows > kNormFewRows ? 1 : 0;
+    config.numAttrs = 1;
     return cudaLaunchKernelEx(&config, kernel, static_cast<const __nv_bfloat16*>(x),
                               static_cast<const R*>(residual), static_cast<const W*>(weight), rows,
                               hidden, eps, static_cast<__nv_bfloat16*>(out), codes, scale,
