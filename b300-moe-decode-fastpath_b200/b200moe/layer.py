@@ -215,7 +215,15 @@ def b300_moe_layer(
     are used unrounded.  ``return_routing=True`` also returns ``(ids [T,K] int64,
     weights [T,K] float32)``.  ``workspace``, ``check_status`` and ``out`` as in
     :func:`b300_moe_forward`, except that ``out`` has to be on the device; it may be the hidden
-    states themselves, which every block has read before the first row is stored.
+    states themselves, which every block has read before the first row is stored.  A workspace
+    serves one call at a time: eager calls on several streams it orders itself, replays of
+    captured calls (and eager calls beside them) are ordered by the caller.
+
+    Against the router's product, :func:`topk_routing` and :func:`b300_moe_forward` in one graph
+    this is 1.03 to 1.8 times as fast for one token and about the same for eight (H = 2048 with 128
+    experts of 768: 25 against 45 us, and 98 against 98 us); outside a graph it also takes one
+    call's host time instead of three.  Pass a workspace that is kept: a call without one
+    allocates the buffers of the whole forward each time.
     """
 
     _check_options(hidden_states, out, return_routing, check_status)
@@ -238,7 +246,14 @@ def b300_moe_layer_fp8(
     out: torch.Tensor | None = None,
 ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """:func:`b300_moe_layer` with the E4M3 expert weights of
-    :func:`quantize_expert_weights_fp8`; H and I multiples of 16."""
+    :func:`quantize_expert_weights_fp8`; H and I multiples of 16.
+
+    Activations between the two products keep 11 significant bits (twelve in
+    :func:`b300_moe_forward_fp8`), scaled by the largest of their row.  One token is 1.1 to 1.5
+    times as fast as through the router's product, :func:`topk_routing` and
+    :func:`b300_moe_forward_fp8` in one graph; from three tokens on with large experts those three
+    are faster (H = I = 2880, 32 experts, three tokens: 103 against 107 us; H = 4096, I = 14336,
+    8 experts, eight tokens: 230 against 246 us)."""
 
     _check_options(hidden_states, out, return_routing, check_status)
     if not isinstance(weights, Fp8ExpertWeights):

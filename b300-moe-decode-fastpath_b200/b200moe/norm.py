@@ -2,8 +2,8 @@
 
 No counterpart in the reference, which starts at the layer's hidden states.  One kernel adds
 the layer input to the residual stream, stores the new residual and writes the normalised rows
-either in BF16 (what :func:`b200moe.b300_moe_forward` and :func:`b200moe.b300_moe_layer` take)
-or as E4M3 codes with one FP32 scale per row, the format of :func:`b200moe.quantize_rows_fp8`.
+either in BF16 (what every layer of this package takes) or, for products of the caller's own, as
+E4M3 codes with one FP32 scale per row, the format of :func:`b200moe.quantize_rows_fp8`.
 """
 
 from __future__ import annotations
@@ -196,7 +196,8 @@ def add_rms_norm_fp8(
     ``codes`` uint8 [..., H] and ``scale`` FP32 [...] follow :func:`quantize_rows_fp8`:
     ``scale = max|row| / 448`` (1 for a row of zeros), ``code = E4M3(value / scale)`` rounded to
     nearest even, taken from the FP32 values, not from their BF16 rounding.  H must be a
-    multiple of 16.
+    multiple of 16.  The rows are for products of the caller's own that take E4M3 operands: the
+    layers of this package take BF16 rows, those of :func:`add_rms_norm`.
     """
 
     rows = _check(hidden_states, residual, weight, eps, 16)

@@ -30,9 +30,9 @@
 // 8 experts, top-2: 118 us (107) and 422 us (412); E4M3 74.5 us (37) and 246 us (206) at the two
 // shapes for eight tokens, 106 us (68) for three with H = I = 2880, 32 experts, top-8, where the
 // 20 output rows of a block fill 32 rows of MMAs (without the MMAs 16 us less, without loading
-// activations 9 us less).  The router's product, top-k and the regular path, in a graph: 45, 98,
-// 125 and 412 to 420 us; E4M3 227 us for eight tokens, 103 us for three, 34 us against 23 us for
-// one token at the first shape, 82 us against 73 us at the second.
+// activations 9 us less).  The router's product, top-k and the regular path, in a graph: 45, 99,
+// 127 and 421 us; E4M3 230 us for eight tokens, 104 us for three, 34 us against 23 us for one token
+// at the first shape, 82 us against 72 us at the second.
 //
 // Loads.  Each lane copies with cp.async the very 16 bytes that it will use as fragments (rows
 // g and g+8, four lanes side by side in a row), into a ring of its warp in shared memory, and

@@ -9,7 +9,7 @@
 // bytes of its operands: x, r, r', y.  Many rows
 // are bound by HBM: 8192 x 4096 in 41.4 us (6.48 TB/s, 0.99 of the measured copy rate), with E4M3
 // result 36.9 us (0.97); 4099 x 2880 E4M3 in 16.0 us (0.79: two waves of short rows).  One row
-// is bound by the latency of one load, one barrier and one store: 1.7 us for 4096 columns.
+// is bound by the latency of one load, one barrier and one store: 1.8 us for 4096 columns.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -216,7 +216,7 @@ cudaError_t launch_norm(const void* x, const void* residual, const void* weight,
   const dim3 grid((unsigned)((rows + together - 1) / together));
   auto run = [&](auto kernel) {
     // The launch overlaps the end of the kernel in front, for which the kernel waits before it
-    // reads anything (1 x 4096: 2.05 -> 1.7 us, 4099 x 2880 16.4 -> 15.8 us, 8192 x 4096 E4M3 38.9
+    // reads anything (1 x 4096: 2.05 -> 1.8 us, 4099 x 2880 16.4 -> 15.8 us, 8192 x 4096 E4M3 38.9
     // -> 38.3 us back to back; 296 x 4096 2.9 -> 3.1 us).
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -22,9 +22,12 @@
 // What bounds it.  Few rows: the chain of load, four to five cluster barriers (0.23 us each, a
 // remote read 0.37 us) and two passes over shared memory: 14.4 us for top-p over 32000 tokens,
 // 13.3 us for 17 rows of 32003 with top-k and top-p, 11.1 us for plain draws from 8 rows of
-// 129280.  Many rows: the FP64 exponentials, twelve operations a token and pass, the integer
-// work around them and the histogram's atomics: 64 rows of 129280 in 34.7 us plain, 75 us with
-// top-p 0.9, 37.6 us with top-k, 48.5 us mixed (5.0 us for the bytes alone).  Shared-memory atomics
+// 129280.  Many rows: the same chain twice, since two blocks to an SM make 1.7 waves of 64 rows
+// of 129280, with passes between its barriers that are chains of dependent operations (twelve in
+// FP64 a token) and atomics: 34.6 us plain, 75.7 us with top-p 0.9, 37.8 us with top-k, 48.5 us
+// mixed (5.0 us for the bytes alone).  Neither arithmetic nor memory is near its limit: with top-p
+// an instruction is issued in 40 % of the cycles, the FP64 pipe is busy in 8 %, DRAM in 5 %, and
+// warps wait for results, for barriers and for shared memory.  Shared-memory atomics
 // of 64 bits are loops of compare-and-swap (9,000 to 16,000 cycles for 16,384 tokens, 240,000
 // where they meet in four bins), those of 32 bits are not (1,300 and 4,300), so a weight is added
 // as three parts of 15 bits.
