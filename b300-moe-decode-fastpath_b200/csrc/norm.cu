@@ -6,10 +6,11 @@
 //
 // A row is read once and stays in registers between the sum of its squares, the largest |y|
 // and the stores (of the longest rows up to 28 bytes a thread do not), so the kernel moves the
-// bytes of its operands: x, r, r', y.  Many rows
-// are bound by HBM: 8192 x 4096 in 41.4 us (6.48 TB/s, 0.99 of the measured copy rate), with E4M3
-// result 36.9 us (0.97); 4099 x 2880 E4M3 in 16.0 us (0.79: two waves of short rows).  One row
-// is bound by the latency of one load, one barrier and one store: 1.8 us for 4096 columns.
+// bytes of its operands: x, r, r', y.  Many rows are bound by HBM: 8192 x 4096 in 40.5 us
+// (6.63 TB/s, 1.01 of the measured copy rate), 4096 x 7168 with FP32 residual and weight 53.4 us
+// (1.00); with E4M3 result 38.3 us (0.93: each element is rounded to a code twice) and 55.2 us
+// (0.89); 4099 x 2880 E4M3 in 16.6 us (0.76: the same, and the start and end of a short kernel).
+// One row is bound by the latency of one load, one barrier and one store: 1.8 us for 4096 columns.
 #include <cuda_fp8.h>
 
 #include <type_traits>
