@@ -45,7 +45,7 @@ extern "C" {
 
 /* bits of the device status word */
 #define B200MOE_STATUS_BAD_EXPERT_ID  0x1u  /* some expert id was outside [0, E); its row was dropped */
-#define B200MOE_STATUS_PIPE_TIMEOUT   0x2u  /* a bounded mbarrier wait inside a GEMM gave up */
+#define B200MOE_STATUS_PIPE_TIMEOUT   0x2u  /* a bounded wait inside a GEMM or the one-kernel layer gave up */
 #define B200MOE_STATUS_PEER_TIMEOUT   0x4u  /* a bounded wait on an expert-parallel peer flag gave up */
 
 #define B200MOE_MAX_EXPERTS   256   /* same limit as the reference, csrc/routing_kernels.cu:107 */
@@ -506,6 +506,8 @@ int b200moe_router_topk(const void* logits, int logits_are_f32, int num_tokens, 
  * grid-barrier counters, which every call leaves at zero, and the status word).  A cooperative
  * launch of one block per SM; one scratch serves one call at a time (stages of a forward on the
  * same scratch included: what they leave there for one another is overwritten).
+ * A barrier wait that runs out (a second) sets B200MOE_STATUS_PIPE_TIMEOUT and leaves the output
+ * unwritten and the counters at zero.
  */
 #define B200MOE_LAYER_MAX_TOKENS 8
 #define B200MOE_LAYER_MAX_HIDDEN 8192
